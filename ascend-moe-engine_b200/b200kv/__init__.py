@@ -80,6 +80,20 @@ class DecodeArgs(Structure):
     ]
 
 
+class SharedArgs(Structure):
+    """b200kv_shared_args (include/b200kv.h)."""
+
+    _fields_ = [
+        ("q", c_void_p), ("q_seq_stride", c_int64), ("q_head_stride", c_int64),
+        ("pool", PoolView),
+        ("block_table", c_void_p), ("max_blocks", c_int64), ("table_rows", c_int64), ("table_index", c_void_p),
+        ("kv_len", c_void_p), ("leader", c_void_p), ("shared_len", c_void_p),
+        ("batch", c_int32), ("heads", c_int32), ("block_size", c_int32), ("scale", c_float),
+        ("out", c_void_p), ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("flags", ctypes.c_uint32),
+        ("out_fp8", c_void_p), ("out_scale", c_void_p),
+    ]
+
+
 class ProducerArgs(Structure):
     """b200kv_producer_args (include/b200kv.h)."""
 
@@ -146,6 +160,13 @@ def _load() -> ctypes.CDLL:
     lib.b200kv_mla_decode.argtypes = [POINTER(DecodeArgs), c_void_p, c_void_p]
     lib.b200kv_mla_decode_static.restype = c_int32
     lib.b200kv_mla_decode_static.argtypes = [POINTER(DecodeArgs), c_void_p, c_void_p]
+    lib.b200kv_mla_decode_shared_workspace_bytes.restype = c_size_t
+    lib.b200kv_mla_decode_shared_workspace_bytes.argtypes = [c_int32, c_int32]
+    lib.b200kv_mla_decode_shared.restype = c_int32
+    lib.b200kv_mla_decode_shared.argtypes = [POINTER(SharedArgs), c_void_p, c_void_p]
+    lib.b200kv_copy_blocks.restype = c_int32
+    lib.b200kv_copy_blocks.argtypes = [POINTER(PoolView), c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                       c_void_p]
     lib.b200kv_append_fused.restype = c_int32
     lib.b200kv_append_fused.argtypes = [POINTER(ProducerArgs), c_void_p, c_void_p]
     lib.b200kv_mx_quant_e4m3.restype = c_int32
@@ -225,7 +246,8 @@ _POOL = f"{ctypes.sizeof(PoolView)}s"
 _pack_decode = struct.Struct(f"@Pqq{_POOL}PqPPiiifPPPPPPNiiPqPqIPqPP").pack
 _pack_producer = struct.Struct(f"@{_POOL}PqPfPqPqPqPqqiPqPqP").pack
 _pack_indexer = struct.Struct("@PPPiPqPqPqPiiqiPPPNiP").pack
-for _pack, _type, _fields in ((_pack_decode, DecodeArgs, 31), (_pack_producer, ProducerArgs, 19), (_pack_indexer, IndexerArgs, 21)):
+_pack_shared = struct.Struct(f"@Pqq{_POOL}PqqPPPPiiifPPPNIPP").pack
+for _pack, _type, _fields in ((_pack_decode, DecodeArgs, 31), (_pack_shared, SharedArgs, 22), (_pack_producer, ProducerArgs, 19), (_pack_indexer, IndexerArgs, 21)):
     assert len(_pack(*(bytes(ctypes.sizeof(PoolView)) if t is PoolView else 0 for _, t in _type._fields_))) == ctypes.sizeof(_type)
 _torch_c = None
 
@@ -239,6 +261,7 @@ def _packed_entry(name: str):
 
 
 _mla_decode, _mla_decode_static = _packed_entry("b200kv_mla_decode"), _packed_entry("b200kv_mla_decode_static")
+_mla_decode_shared = _packed_entry("b200kv_mla_decode_shared")
 _append_fused, _indexer_topk = _packed_entry("b200kv_append_fused"), _packed_entry("b200kv_indexer_topk")
 
 
@@ -335,6 +358,14 @@ def gather(view: PoolView, block_table, kv_len, block_size: int, out_latent, out
                             _stream_handle(stream), _ptr(status)))
 
 
+def copy_blocks(view: PoolView, moves, block_size: int, layers: int = 1, latent_layer_stride: int = 0, rope_layer_stride: int = 0,
+                status=None, stream=None) -> None:
+    """Pages copied inside the cache, in every layer at once: moves int32 [n, 3] on the device, (source block, destination block,
+    rows) each. `view` is layer 0's; the strides lead from one layer to the next, in elements."""
+    check(lib.b200kv_copy_blocks(ctypes.byref(view), layers, latent_layer_stride, rope_layer_stride, moves.data_ptr(), moves.shape[0], block_size,
+                                 _stream_handle(stream), _ptr(status)))
+
+
 def indexer_topk(q_fp8, q_scale, weights, key_pool, k_scale, block_table, kv_len, block_size: int, max_kv_len: int,
                  k: int, status=None, stream=None, variant: int = INDEXER_AUTO, scores_out=None, rows_out=None):
     """The k best-scoring tokens of every sequence: q_fp8 uint8 [B, H, 128], q_scale fp32 [B, H], weights bf16
@@ -423,6 +454,26 @@ def mla_decode_static(q, view: PoolView, block_table, kv_len, block_size: int, s
     workspace tensor; nothing is allocated on the device by the call."""
     args = _decode_args(q, view, block_table, kv_len, block_size, scale, out, lse, kv_begin, None, max_ctas, False, partial)
     check(_mla_decode_static(args, _stream_handle(stream), _ptr(status)))
+
+
+def decode_shared_workspace_bytes(batch: int, heads: int = HEADS) -> int:
+    return int(lib.b200kv_mla_decode_shared_workspace_bytes(batch, heads))
+
+
+def mla_decode_shared(q, view: PoolView, block_table, kv_len, block_size: int, scale: float, leader, shared_len, table_index=None,
+                      out=None, lse=None, workspace=None, status=None, stream=None, stable_tables: bool = False, quantised=None) -> None:
+    """Decode attention of queries that share rows of the cache: q bf16 [B, H, 576], kv_len int32 [B] as in mla_decode; consecutive
+    queries with the same leader int32 [B] (the index of the first of them) have the same blocks for their first shared_len int32
+    [B] tokens. table_index int32 [B]: each query's row of block_table (None: row b for query b); the tokens of one sequence, each
+    attending up to itself, have one row and a shared_len of the longest kv_len."""
+    batch, heads = q.shape[:2]
+    q_seq_stride, q_head_stride = q.stride()[:2]
+    ws, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+    fp8, scales = (0, 0) if quantised is None else (_ptr(quantised[0]), _ptr(quantised[1]))
+    args = _pack_shared(q.data_ptr(), q_seq_stride, q_head_stride, bytes(view) if isinstance(view, PoolView) else _refuse_view(view), _ptr(block_table),
+                        block_table.stride()[0], block_table.shape[0], _ptr(table_index), _ptr(kv_len), _ptr(leader), _ptr(shared_len), batch, heads,
+                        block_size, scale, _ptr(out), _ptr(lse), ws, ws_bytes, 1 if stable_tables else 0, fp8, scales)
+    check(_mla_decode_shared(args, _stream_handle(stream), _ptr(status)))
 
 
 def lse_merge(partial_o, partial_m, partial_l, out, lse=None, stream=None) -> None:

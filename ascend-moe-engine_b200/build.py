@@ -20,9 +20,9 @@ OUT = os.path.join(HERE, "b200kv", "libb200kv.so")
 
 SOURCES = [
     "capi.cu",
-    "kv_move.cu", "kv_gather_tma.cu",
+    "kv_move.cu", "kv_gather_tma.cu", "kv_pages.cu",
     "mla_decode_simt.cu",
-    "mla_decode_tc.cu", "mla_decode_cluster.cu",
+    "mla_decode_tc.cu", "mla_decode_cluster.cu", "mla_decode_shared.cu",
     "kv_block_pool.cpp",
     "kv_arena.cpp",
     "kv_partition.cpp",

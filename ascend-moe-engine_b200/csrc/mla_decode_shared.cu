@@ -1,0 +1,1102 @@
+// Decode attention of queries that share rows of the cache, on tcgen05 tensor cores (sm_100a), 64 heads x (512 + 64).
+//
+// Sequences forked from one prompt, the draft tokens of a step and the tokens of a prompt's chunk attend over the same rows.
+// With 64 heads a row of 1,152 bytes is worth 139,264 operations a query: from two queries on the tensor cores are the bound and
+// not HBM, so the work is arranged around them. Two queries (128 rows of S) and a pair of CTAs belong together:
+//
+//   S   [128 rows x 64 tokens]    each CTA for ITS 64 of a step's 128 tokens:  Q (A) x K^T (B), M = 128 N = 64, 36 k-steps;
+//   P   = exp2(S * scale * log2e - m), bf16, written to shared memory and copied into the other CTA's;
+//   O^T [256 columns x 128 rows]  each CTA for ITS half of the 512 value columns, over all 128 tokens: V^T (A) x P^T (B),
+//                                 M = 128 N = 128, 2 x 8 k-steps.
+//
+// So each of the 128 x 512 sums lives in one CTA's tensor memory (a whole O would fill it and leave no room for S), nothing is
+// computed twice, every MMA has M = 128, and the tokens' rows that a CTA takes in are its own 64 x 576 and the other's
+// 64 x 256. Q does not fit beside them in shared memory: two thirds of it lie in tensor memory as the A operand, which also
+// halves what those MMAs read of shared memory. Tensor memory: O^T 256 columns, S 64, Q 192: all 512.
+//
+// The two CTAs keep one running maximum: each sends its 128 rows' maxima over its tokens to the other before it exponentiates
+// (one asynchronous 4-byte store a thread), and both come to the same reference. As in the other kernels O is rescaled only when
+// the maximum grows by more than 2^8, so the rounding of P to bf16 (relative 2^-9 of every weight, unbiased; sums and the
+// log-sum-exp take the unrounded fp32 weights) is the only one below fp32.
+//
+// The list of work. A pair of queries is an item of n steps: first the tokens that both share (or a prefix of them: the tokens
+// of one sequence each attend up to themselves), then the first query's own tokens, then the second's, all into the same
+// accumulators; in the latter, only that query's 64 rows of P take part. All items' steps form one flat list, cut into one run
+// per CTA pair by cost; a run's first and last item may be cut, and then leave fp32 partials (m, l, O) in the workspace which
+// the second kernel merges. A tile of tokens that is complete for one of the two queries only is two steps, one per query,
+// so that a NaN or an infinity in a row behind a query's end never meets that query's weights (0 x NaN).
+//
+// Warps 0-3: softmax and epilogue (thread = row), 4 and 7: loads, 5: QK, 6: PV. Every wait is bounded; the CTAs of a pair leave
+// together through the cluster barrier.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "mla_tc_common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace b200kv {
+
+int32_t ValidatePoolView(const b200kv_pool_view* pool);
+int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, CUtensorMap* out);
+int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t box_heads,
+                CUtensorMap* out);
+
+namespace {
+
+using namespace mla;
+
+constexpr int kThreads = 256;
+constexpr int kRows = 2 * kHeads;   // two queries
+constexpr int kStep = 2 * kTile;    // tokens of a step: a tile for each CTA of the pair
+constexpr int kHalf = kLatent / 2;  // value columns of a CTA
+// K slabs of 64 columns: those of the CTA's own half of the value columns ("V", four), the other four and the rope ("T", five).
+// Q's slabs in the same order: T0, T1 and V0-V3 in tensor memory, T2, T3 and the rope in shared memory.
+constexpr int kTSlabs = 5, kVSlabs = 4, kQSmemSlabs = 3, kQTmemSlabs = 6;
+constexpr int kQSlab = kRows * 128;  // 16,384
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320;
+static_assert(kColQ + kQTmemSlabs * 32 == kTmemCols, "tensor memory is full");
+
+// Shared memory (offsets from a 1024-byte aligned base).
+constexpr int kOffQ = 0;
+constexpr int kOffT = kOffQ + kQSmemSlabs * kQSlab;
+constexpr int kOffV = kOffT + kTSlabs * kSlabBytes;           // two sets: PV of a step reads one while the next step's QK reads the other
+constexpr int kOffW = kOffV + 2 * kVSlabs * kSlabBytes;       // the other CTA's tokens, this CTA's columns
+constexpr int kOffP = kOffW + kVSlabs * kSlabBytes;           // weights of this CTA's tokens
+constexpr int kPBytes = kRows * 128;
+constexpr int kOffPeerP = kOffP + kPBytes;                    // weights of the other CTA's tokens
+constexpr int kOffMisc = kOffPeerP + kPBytes;
+constexpr int kMiscBytes = 4096;
+constexpr int kSmemBytes = kOffMisc + kMiscBytes + 1024;
+static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
+
+struct Misc {
+  uint64_t t_full, t_empty;
+  // V and W come and go in halves of two slabs, the 128 columns of one accumulator: PV gives the first half back half way.
+  uint64_t v_full[2][2], v_empty[2][2];  // [set][half]
+  uint64_t w_full[2], w_empty[2];
+  uint64_t q_full, q_empty;    // the slabs in shared memory
+  uint64_t qt_full;            // the slabs in tensor memory
+  uint64_t s_full, s_empty;
+  uint64_t p_full;             // own weights written, rows behind the end zeroed
+  uint64_t peer_p_full;        // the other CTA's weights have landed
+  uint64_t pv_done;            // both CTAs' PV of a step are complete: the weights may be overwritten
+  uint64_t o_empty;
+  uint64_t max_full[2][kSoftmaxWarps];
+  uint64_t drain[2];
+  uint32_t tmem_base;
+  int32_t abort_flag;
+  int32_t start_query;  // the run's first item, the step in it, and how many steps
+  int32_t start_step;
+  int32_t n_steps;
+  unsigned long long flat_lo, flat_hi;
+  unsigned long long scan[8][2];
+  float peer_max[2][kRows];
+  float factor[kRows];
+};
+static_assert(sizeof(Misc) <= kMiscBytes, "Misc does not fit its reservation");
+
+struct SharedParams {
+  const __nv_bfloat16* q;
+  int64_t q_seq_stride;
+  int64_t q_head_stride;
+  const int32_t* block_table;
+  int64_t max_blocks;
+  int64_t table_rows;
+  const int32_t* table_index;
+  const int32_t* kv_len;
+  const int32_t* leader;
+  const int32_t* shared_len;
+  int64_t pool_rows;
+  int32_t batch;
+  int32_t block_size;
+  int32_t stable_tables;
+  float scale_log2;
+  double natural;  // scale / scale_log2: from the kernels' log2 domain back to natural logarithms
+  __nv_bfloat16* out;
+  float* lse;
+  // Partials: slot 2c of run c is an item it continues, slot 2c + 1 one it begins and does not finish. O as [slot][32 row
+  // quads][512 columns][4 rows]: an epilogue thread owns a column and has its rows in consecutive registers.
+  float* ws_o;
+  float* ws_m;  // [slot][128], log2 domain
+  float* ws_l;
+  int32_t* first_run;  // [batch], by an item's first query: the runs that hold its first and its last step
+  int32_t* last_run;
+  int32_t* has_steps;  // [runs]
+  int32_t* status;
+};
+
+// ---- the list of work -------------------------------------------------------------------------------------------------
+// Query b is the second of a pair if the one before it has the same leader and stands at an even distance from it. What the
+// arrays hold, every query belongs to exactly one item.
+__device__ __forceinline__ bool IsSecond(const int32_t* leader, int b) {
+  return b > 0 && leader[b] == leader[b - 1] && ((static_cast<unsigned>(b - 1) - static_cast<unsigned>(leader[b - 1])) & 1u) == 0;
+}
+
+struct Item {
+  int q0, q1;        // q1 < 0: a query alone
+  int len0, len1;
+  int lim0, lim1;    // tokens of the common part that each query attends over
+  int own;           // where the own tokens begin
+  int split;         // common tile that is two steps, or -1
+  int common, own0, own1;  // steps
+  __device__ __forceinline__ int steps() const { return common + own0 + own1; }
+};
+
+__device__ __forceinline__ int StepsOf(int tokens) { return tokens > 0 ? (tokens - 1) / kStep + 1 : 0; }
+
+__device__ __forceinline__ Item MakeItem(int q0, int q1, int len0, int len1, int shared0, int shared1) {
+  Item it;
+  it.q0 = q0;
+  it.q1 = q1;
+  it.len0 = max(len0, 0);
+  it.len1 = q1 >= 0 ? max(len1, 0) : 0;
+  it.split = -1;
+  it.own0 = it.own1 = 0;
+  it.own = 0;
+  if (q1 < 0) {
+    it.lim0 = it.len0;
+    it.lim1 = 0;
+    it.common = StepsOf(it.len0);
+    return it;
+  }
+  const int shared = max(min(shared0, shared1), 0);
+  it.own = shared & ~(kTile - 1);  // (a tile is 64 consecutive rows of a block)
+  it.lim0 = it.len0 <= shared ? it.len0 : it.own;
+  it.lim1 = it.len1 <= shared ? it.len1 : it.own;
+  const int less = min(it.lim0, it.lim1);
+  it.common = StepsOf(max(it.lim0, it.lim1));
+  if (it.lim0 != it.lim1 && (less & (kStep - 1)) != 0) {
+    it.split = less / kStep;
+    ++it.common;
+  }
+  if (it.len0 > shared) it.own0 = StepsOf(it.len0 - it.own);
+  if (it.len1 > shared) it.own1 = StepsOf(it.len1 - it.own);
+  return it;
+}
+
+__device__ __forceinline__ Item ItemAt(const SharedParams& p, int b) {  // b: not a second
+  const bool pair = b + 1 < p.batch && IsSecond(p.leader, b + 1);
+  return MakeItem(b, pair ? b + 1 : -1, p.kv_len[b], pair ? p.kv_len[b + 1] : 0, p.shared_len[b], pair ? p.shared_len[b + 1] : 0);
+}
+
+struct Step {
+  int query;   // whose table row
+  int token;   // first token
+  int valid;   // 1 .. 128 tokens
+  int active;  // bit 0: the first query's rows, bit 1: the second's
+};
+
+__device__ __forceinline__ Step StepAt(const Item& it, int s) {
+  Step st;
+  if (s < it.common) {
+    int tile = s;
+    st.query = it.q0;
+    if (it.split >= 0 && s > it.split) --tile;
+    st.token = tile * kStep;
+    const int in0 = it.lim0 - st.token, in1 = it.lim1 - st.token;
+    if (it.split >= 0 && tile == it.split) {  // first the query that ends in this tile, then the other
+      const bool first_ends = it.lim0 < it.lim1;
+      st.active = (s == it.split) == first_ends ? 1 : 2;
+    } else {
+      st.active = (in0 > 0 ? 1 : 0) | (in1 > 0 ? 2 : 0);
+    }
+    st.valid = min(kStep, st.active == 1 ? in0 : st.active == 2 ? in1 : min(in0, in1));
+    return st;
+  }
+  s -= it.common;
+  const bool second = s >= it.own0;
+  if (second) s -= it.own0;
+  st.query = second ? it.q1 : it.q0;
+  st.token = it.own + s * kStep;
+  st.active = second ? 2 : 1;
+  st.valid = min(kStep, (second ? it.len1 : it.len0) - st.token);
+  return st;
+}
+
+// The cut: a step costs 2, entering another item in mid-run 3 more (Q is loaded anew and the accumulators are drained). Step x
+// of the flat list, of the item with ordinal s, stands at cost position 2x + 3s; run c takes the positions
+// [ceil(c C / G), ceil((c + 1) C / G)).
+struct Cut {
+  long long total_cost;
+  long long runs;
+  static constexpr long long kStepCost = 2, kEnterCost = 3;
+  __device__ static long long Pos(long long x, long long s) { return kStepCost * x + kEnterCost * s; }
+  __device__ long long First(long long c) const { return (c * total_cost + runs - 1) / runs; }
+};
+
+// The items of this run, one after the other. Every role runs the same walk.
+struct Walk {
+  const SharedParams& p;
+  int query;
+  int step;
+  int remaining;
+  __device__ Walk(const SharedParams& params, const Misc* misc)
+      : p(params), query(misc->start_query), step(misc->start_step), remaining(misc->n_steps) {}
+  __device__ bool Next(Item* item, int* lo, int* hi) {
+    while (remaining > 0 && query < p.batch) {
+      if (!IsSecond(p.leader, query)) {
+        const Item it = ItemAt(p, query);
+        const int n = it.steps();
+        if (step < n) {
+          const int take = min(remaining, n - step);
+          *item = it;
+          *lo = step;
+          *hi = step + take;
+          remaining -= take;
+          step = 0;
+          ++query;  // (an item that is not finished here is the run's last)
+          return true;
+        }
+      }
+      step = 0;
+      ++query;
+    }
+    return false;
+  }
+};
+
+// A bounded wait by all lanes of a warp together, behind an inline probe.
+__device__ __forceinline__ bool WarpWait(uint32_t bar, uint32_t parity, Misc* misc, int32_t* status, int site) {
+  if (__all_sync(0xffffffffu, ptx::MbarTestWait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, BoundedWait(bar, parity, misc, status, site));
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    MlaDecodeSharedKernel(const __grid_constant__ CUtensorMap latent_map, const __grid_constant__ CUtensorMap rope_map,
+                          const __grid_constant__ CUtensorMap q_map, const __grid_constant__ SharedParams p) {
+  extern __shared__ unsigned char smem_dyn[];
+  const uint32_t raw = ptx::SmemAddr(smem_dyn);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  unsigned char* smem = smem_dyn + (base - raw);
+  Misc* misc = reinterpret_cast<Misc*>(smem + kOffMisc);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1;
+  const int run = blockIdx.x >> 1;
+  const int runs = gridDim.x >> 1;
+  auto bar = [&](const uint64_t* b) { return ptx::SmemAddr(b); };
+
+  if (threadIdx.x == 0) {
+    ptx::MbarInit(bar(&misc->t_full), 1);
+    ptx::MbarInit(bar(&misc->t_empty), 1);
+    for (int s = 0; s < 2; ++s) {
+      for (int h = 0; h < 2; ++h) {
+        ptx::MbarInit(bar(&misc->v_full[s][h]), 1);
+        ptx::MbarInit(bar(&misc->v_empty[s][h]), 1);
+      }
+      ptx::MbarInit(bar(&misc->w_full[s]), 1);
+      ptx::MbarInit(bar(&misc->w_empty[s]), 1);
+      ptx::MbarInit(bar(&misc->drain[s]), 1);
+      for (int w = 0; w < kSoftmaxWarps; ++w) ptx::MbarInit(bar(&misc->max_full[s][w]), 1);
+    }
+    ptx::MbarInit(bar(&misc->q_full), 1);
+    ptx::MbarInit(bar(&misc->q_empty), 1);
+    ptx::MbarInit(bar(&misc->qt_full), kSoftmaxWarps);
+    ptx::MbarInit(bar(&misc->s_full), 1);
+    ptx::MbarInit(bar(&misc->s_empty), kSoftmaxWarps);
+    ptx::MbarInit(bar(&misc->p_full), kSoftmaxWarps);
+    ptx::MbarInit(bar(&misc->peer_p_full), 1);
+    ptx::MbarInit(bar(&misc->pv_done), 2);
+    ptx::MbarInit(bar(&misc->o_empty), kSoftmaxWarps);
+    misc->abort_flag = 0;
+    misc->start_query = p.batch;
+    misc->start_step = 0;
+    misc->n_steps = 0;
+    ptx::FenceBarrierInit();
+    ptx::PrefetchTensorMap(&latent_map);
+    ptx::PrefetchTensorMap(&rope_map);
+    ptx::PrefetchTensorMap(&q_map);
+  }
+  if (warp == 5) {
+    ptx::TmemAlloc(ptx::SmemAddr(&misc->tmem_base), kTmemCols);
+    ptx::TmemRelinquish();
+  }
+  __syncwarp();
+  ptx::ClusterArrive();  // (the barriers are ready: waited for before the peer's are touched)
+  if (p.stable_tables == 0) GridDependencyWait();
+  // (let go only after this kernel's own wait: the merge kernel reads the lengths too)
+
+  // ---- this run of the list: totals, then the first step at or after the run's first cost position and the next run's ------
+  {
+    unsigned long long steps = 0, items = 0;
+    for (int b = threadIdx.x; b < p.batch; b += kThreads) {
+      const int n = IsSecond(p.leader, b) ? 0 : ItemAt(p, b).steps();
+      steps += n;
+      items += n > 0 ? 1 : 0;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      steps += __shfl_xor_sync(0xffffffffu, steps, off);
+      items += __shfl_xor_sync(0xffffffffu, items, off);
+    }
+    if (lane == 0) {
+      misc->scan[warp][0] = steps;
+      misc->scan[warp][1] = items;
+    }
+    __syncthreads();
+    long long total = 0, total_items = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      total += misc->scan[w][0];
+      total_items += misc->scan[w][1];
+    }
+    if (threadIdx.x == 0) {
+      misc->flat_lo = total;
+      misc->flat_hi = total;
+    }
+    const Cut cut{Cut::Pos(total, total_items > 0 ? total_items - 1 : 0), runs};
+    const long long k_lo = cut.First(run), k_hi = cut.First(run + 1);
+    long long before = 0, before_items = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+      __syncthreads();
+      const int b = b0 + threadIdx.x;
+      const int n = b < p.batch && !IsSecond(p.leader, b) ? ItemAt(p, b).steps() : 0;
+      long long incl = n, incl_items = n > 0 ? 1 : 0;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, off);
+        const long long up_items = __shfl_up_sync(0xffffffffu, incl_items, off);
+        if (lane >= off) {
+          incl += up;
+          incl_items += up_items;
+        }
+      }
+      if (lane == 31) {
+        misc->scan[warp][0] = incl;
+        misc->scan[warp][1] = incl_items;
+      }
+      __syncthreads();
+      long long chunk = 0, chunk_items = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) {
+          incl += misc->scan[w][0];
+          incl_items += misc->scan[w][1];
+        }
+        chunk += misc->scan[w][0];
+        chunk_items += misc->scan[w][1];
+      }
+      if (n > 0) {
+        const long long first = before + incl - n, s = before_items + incl_items - 1;
+        const long long last_pos = Cut::Pos(first + n - 1, s);
+        const long long last_before = Cut::Pos(first - 1, s - 1);  // the item before this one ends here
+        auto at_or_after = [&](long long k) {                      // first step at or after cost position k, if it is in this item
+          const long long x = (k - Cut::kEnterCost * s + 1) >> 1;
+          return x > first ? x : first;
+        };
+        if (last_pos >= k_lo && (s == 0 || last_before < k_lo)) {
+          const long long x = at_or_after(k_lo);
+          misc->flat_lo = x;
+          misc->start_query = b;
+          misc->start_step = static_cast<int>(x - first);
+        }
+        if (last_pos >= k_hi && (s == 0 || last_before < k_hi)) misc->flat_hi = at_or_after(k_hi);
+      }
+      before += chunk;
+      before_items += chunk_items;
+    }
+  }
+  ptx::TcFenceBeforeSync();
+  __syncthreads();
+  ptx::TcFenceAfterSync();
+  if (threadIdx.x == 0) misc->n_steps = static_cast<int>(misc->flat_hi - misc->flat_lo);
+  if (p.stable_tables != 0) GridDependencyWait();
+  GridDependencyTrigger();
+  __syncthreads();
+  ptx::ClusterWait();
+  if (threadIdx.x == 0 && rank == 0) p.has_steps[run] = misc->n_steps > 0 ? 1 : 0;
+
+  const uint32_t tmem = misc->tmem_base;
+  bool ok = true;
+
+  if (warp == 4 || warp == 7) {
+    // ======================= loads ============================================================================
+    // Warp 4 brings a step's T and V (and Q), warp 7 its W, which waits for the PV before: in one warp that wait would hold the
+    // next step's T back.
+    // Pool row of a tile, through the block table; the row behind the pool (which loads as zeros) for a tile without tokens and
+    // for a bad entry, which is recorded.
+    auto tile_row = [&](const Step& st, int tile) -> int32_t {
+      const int in_step = tile * kTile;
+      if (in_step >= st.valid) return static_cast<int32_t>(p.pool_rows);
+      const int token = st.token + in_step;
+      const int64_t table_row = p.table_index != nullptr ? p.table_index[st.query] : st.query;
+      const int64_t column = token / p.block_size;
+      const bool inside = table_row >= 0 && table_row < p.table_rows && column < p.max_blocks;
+      const int64_t block = inside ? p.block_table[table_row * p.max_blocks + column] : -1;
+      const int64_t row = block * p.block_size + token % p.block_size;
+      if (block < 0 || row + kTile > p.pool_rows) {
+        RecordError(p.status, B200KV_DEV_BAD_BLOCK, st.query, static_cast<int32_t>(column), static_cast<int32_t>(block));
+        return static_cast<int32_t>(p.pool_rows);
+      }
+      return static_cast<int32_t>(row);
+    };
+    // Warp 4, lane l < 5: slab T(l); l < 9: V(l - 5). Warp 7, lane l < 4: the other tile's slab of the same columns as V(l).
+    const bool is_w = warp == 7, is_t = !is_w && lane < kTSlabs;
+    const bool loader = lane < (is_w ? kVSlabs : kTSlabs + kVSlabs);
+    const int j = is_t || is_w ? lane : lane - kTSlabs;
+    const int column = 64 * (is_t ? kVSlabs * (1 - rank) + j : kVSlabs * rank + j);  // (T4 is the rope slab)
+    const bool announces = is_t ? j == 0 : (j & 1) == 0;
+    const uint32_t announced = (is_t ? kTSlabs : 2) * kSlabBytes;
+    const int half = is_t ? 0 : (j >> 1) & 1;
+    const uint32_t dst0 = base + (is_t ? kOffT : is_w ? kOffW : kOffV) + j * kSlabBytes;
+    Walk walk(p, misc);
+    Item item;
+    int lo, hi;
+    int g = 0, seg = 0;
+    while (ok && walk.Next(&item, &lo, &hi)) {
+      if (!is_w) {
+        if (seg > 0) ok = WarpWait(bar(&misc->q_empty), (seg - 1) & 1, misc, p.status, 11);
+        if (!ok) break;
+        if (lane < 2 * kQSmemSlabs) {  // Q's slabs in shared memory: T2, T3, rope; a box of 64 heads each for both queries
+          const int slab = lane >> 1, which = lane & 1;
+          const int query = which == 0 ? item.q0 : item.q1;
+          const uint32_t full = bar(&misc->q_full);
+          if (lane == 0) ptx::MbarArriveExpectTx(full, kQSmemSlabs * kQSlabBytes * (item.q1 >= 0 ? 2 : 1));
+          if (query >= 0) {
+            const int x = slab == 2 ? kLatent : 64 * (kVSlabs * (1 - rank) + 2 + slab);
+            ptx::TmaLoad3D(base + kOffQ + slab * kQSlab + which * kQSlabBytes, &q_map, x, 0, query, full);
+          }
+        }
+        ++seg;
+      }
+      for (int s = lo; s < hi; ++s, ++g) {
+        const int32_t row = tile_row(StepAt(item, s), is_w ? 1 - rank : rank);
+        const int set = g & 1;
+        const uint32_t full = is_t ? bar(&misc->t_full) : is_w ? bar(&misc->w_full[half]) : bar(&misc->v_full[set][half]);
+        const uint32_t empty = is_t ? bar(&misc->t_empty) : is_w ? bar(&misc->w_empty[half]) : bar(&misc->v_empty[set][half]);
+        const uint32_t dst = dst0 + (!is_t && !is_w ? set * kVSlabs * kSlabBytes : 0);
+        // Phase of the buffer's last use: T and W are used every step, a V set every other.
+        const bool every = is_t || is_w;
+        const bool first_use = every ? g < 1 : g < 2;
+        const uint32_t parity = every ? (g & 1) ^ 1 : ((g >> 1) & 1) ^ 1;
+        // The warp polls together; a lane issues its slab the moment its buffer has been given back.
+        bool done = !loader;
+        uint64_t start = 0;
+        for (uint32_t it = 0;; ++it) {
+          if (!done && (first_use || ptx::MbarTestWait(empty, parity))) {
+            if (announces) ptx::MbarArriveExpectTx(full, announced);
+            if (is_t && j == kTSlabs - 1) {
+              ptx::TmaLoad2D(dst, &rope_map, 0, row, full);
+            } else {
+              ptx::TmaLoad2D(dst, &latent_map, column, row, full);
+            }
+            done = true;
+          }
+          if (__all_sync(0xffffffffu, done)) break;
+          if ((it & 1023u) == 1023u) {
+            const uint64_t now = ptx::GlobalTimerNs();
+            if (start == 0) start = now;
+            if (Aborting(misc) || now - start > 1000000000ull) {
+              if (!Aborting(misc) && lane == 0) RaiseTimeout(misc, p.status, 10, parity);
+              ok = false;
+              break;
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+    }
+  } else if (warp == 5) {
+    // ======================= QK ================================================================================
+    constexpr uint32_t kIdesc = ptx::InstrDescBf16(kRows, kTile, 0, 0);
+    const uint64_t q_desc = ptx::SmemDescSw128(base + kOffQ, 16, 1024);
+    const uint64_t t_desc = ptx::SmemDescSw128(base + kOffT, 16, 1024);
+    const uint64_t v_desc0 = ptx::SmemDescSw128(base + kOffV, 16, 1024);
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t d = tmem_u + kColS;
+    Walk walk(p, misc);
+    Item item;
+    int lo, hi;
+    int g = 0, seg = 0;
+    while (ok) {
+      const int have = walk.Next(&item, &lo, &hi) ? 1 : 0;
+      if (__shfl_sync(0xffffffffu, have, 0) == 0) break;
+      const int n = __shfl_sync(0xffffffffu, hi - lo, 0);
+      for (int i = 0; i < n && ok; ++i, ++g) {
+        if (i == 0) {
+          ok = WarpWait(bar(&misc->q_full), seg & 1, misc, p.status, 22) && WarpWait(bar(&misc->qt_full), seg & 1, misc, p.status, 23);
+        }
+        if (ok && g > 0) ok = WarpWait(bar(&misc->s_empty), (g & 1) ^ 1, misc, p.status, 25);
+        if (ok) ok = WarpWait(bar(&misc->t_full), g & 1, misc, p.status, 24);
+        if (!ok) break;
+        ptx::TcFenceAfterSync();
+#pragma unroll
+        for (int k = 0; k < 4 * kTSlabs; ++k) {
+          const int slab = k >> 2, kk = k & 3;
+          const uint64_t b = DescAt(t_desc, slab * kSlabBytes + kk * 32);
+          if (ptx::ElectOne()) {
+            if (slab < 2) {
+              ptx::MmaF16TS(d, tmem_u + kColQ + slab * 32 + kk * 8, b, kIdesc, k > 0 ? 1u : 0u);
+            } else {
+              ptx::MmaF16SS(d, DescAt(q_desc, (slab - 2) * kQSlab + kk * 32), b, kIdesc, 1u);
+            }
+          }
+        }
+        if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty));
+        const int set = __shfl_sync(0xffffffffu, g & 1, 0);
+        const uint64_t v_desc = DescAt(v_desc0, set * kVSlabs * kSlabBytes);
+#pragma unroll
+        for (int half = 0; half < 2 && ok; ++half) {
+          ok = WarpWait(bar(&misc->v_full[set][half]), (g >> 1) & 1, misc, p.status, 26);
+          if (!ok) break;
+          ptx::TcFenceAfterSync();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int slab = 2 * half + (k >> 2), kk = k & 3;
+            if (ptx::ElectOne()) {
+              ptx::MmaF16TS(d, tmem_u + kColQ + (2 + slab) * 32 + kk * 8, DescAt(v_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
+            }
+          }
+        }
+        if (!ok) break;
+        if (ptx::ElectOne()) {
+          ptx::TcCommit(bar(&misc->s_full));
+          if (i == n - 1) ptx::TcCommit(bar(&misc->q_empty));
+        }
+      }
+      ++seg;
+    }
+    if (ptx::ElectOne()) {  // nothing of this warp's may be in flight when tensor memory is freed
+      ptx::TcCommit(bar(&misc->drain[0]));
+      const uint64_t t0 = ptx::GlobalTimerNs();
+      while (!ptx::MbarTryWait(bar(&misc->drain[0]), 0)) {
+        if (ptx::GlobalTimerNs() - t0 > 200000000ull) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    // ======================= PV ================================================================================
+    constexpr uint32_t kIdescBoth = ptx::InstrDescBf16(128, kRows, 1, 0);
+    constexpr uint32_t kIdescOne = ptx::InstrDescBf16(128, kHeads, 1, 0);
+    const uint64_t p_desc = ptx::SmemDescSw128(base + kOffP, 16, 1024);  // K-major: row = row of P, 32 bytes a k-step
+    const uint64_t peer_p_desc = DescAt(p_desc, kOffPeerP - kOffP);
+    const uint64_t v_desc0 = ptx::SmemDescSw128(base + kOffV, kSlabBytes, 1024);  // MN-major: next 64 columns a slab further
+    const uint64_t w_desc = DescAt(v_desc0, kOffW - kOffV);
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+    Walk walk(p, misc);
+    Item item;
+    int lo, hi;
+    int g = 0, seg = 0;
+    while (ok) {
+      const int have = walk.Next(&item, &lo, &hi) ? 1 : 0;
+      if (__shfl_sync(0xffffffffu, have, 0) == 0) break;
+      if (seg > 0) ok = WarpWait(bar(&misc->o_empty), (seg - 1) & 1, misc, p.status, 27);
+      int started = 0;  // queries whose accumulators hold something
+      for (int s = lo; s < hi && ok; ++s, ++g) {
+        const int active = __shfl_sync(0xffffffffu, StepAt(item, s).active, 0);
+        if (ptx::ElectOne()) ptx::MbarArriveExpectTx(bar(&misc->peer_p_full), kPBytes);
+        ok = WarpWait(bar(&misc->w_full[0]), g & 1, misc, p.status, 28) && WarpWait(bar(&misc->w_full[1]), g & 1, misc, p.status, 28) &&
+             WarpWait(bar(&misc->p_full), g & 1, misc, p.status, 21) && WarpWait(bar(&misc->peer_p_full), g & 1, misc, p.status, 29);
+        if (!ok) break;
+        ptx::TcFenceAfterSync();
+        const int set = __shfl_sync(0xffffffffu, g & 1, 0);
+        const uint64_t v_desc = DescAt(v_desc0, set * kVSlabs * kSlabBytes);
+        // Both queries' rows in one pass, or (one of them takes no part, or has begun and the other has not) a pass of 64.
+        const bool one_pass = active == 3 && (started == 0 || started == 3);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          for (int pass = 0; pass < 2; ++pass) {
+            if (one_pass ? pass == 1 : (active >> pass & 1) == 0) continue;
+            const uint32_t idesc = one_pass ? kIdescBoth : kIdescOne;
+            const uint32_t at = one_pass ? 0 : pass * kHeads;  // first row
+            const uint32_t keep = (started >> pass) & 1;
+            const uint64_t pd = DescAt(p_desc, at * 128), ppd = DescAt(peer_p_desc, at * 128);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {  // four k-steps of this CTA's tokens, four of the other's
+              const uint64_t a = DescAt(k < 4 ? v_desc : w_desc, 2 * m * kSlabBytes + (k & 3) * 2048);
+              const uint64_t b = DescAt(k < 4 ? pd : ppd, (k & 3) * 32);
+              if (ptx::ElectOne()) ptx::MmaF16SS(tmem_u + kColO + 128 * m + at, a, b, idesc, k > 0 ? 1u : keep);
+            }
+          }
+          if (ptx::ElectOne()) {
+            if (m == 1) ptx::TcCommitTo(bar(&misc->pv_done), 3);
+            ptx::TcCommit(bar(&misc->v_empty[set][m]));
+            ptx::TcCommit(bar(&misc->w_empty[m]));
+          }
+        }
+        started |= active;
+      }
+      ++seg;
+    }
+    if (ptx::ElectOne()) {
+      ptx::TcCommit(bar(&misc->drain[1]));
+      const uint64_t t0 = ptx::GlobalTimerNs();
+      while (!ptx::MbarTryWait(bar(&misc->drain[1]), 0)) {
+        if (ptx::GlobalTimerNs() - t0 > 200000000ull) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp < kSoftmaxWarps) {
+    // ======================= softmax + epilogue: thread = row ====================================================
+    const int row = threadIdx.x;
+    const int which = row >> 6, head = row & (kHeads - 1);
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t peer = rank ^ 1;
+    const uint32_t peer_max_at = ptx::MapToRank(ptx::SmemAddr(&misc->peer_max[0][row]), peer);
+    const uint32_t peer_max_bar = ptx::MapToRank(bar(&misc->max_full[0][warp]), peer);
+    const uint32_t p_row = base + kOffP + row * 128;
+    const uint32_t p_warp = base + kOffP + warp * 32 * 128;
+    const uint32_t peer_p_warp = ptx::MapToRank(base + kOffPeerP + warp * 32 * 128, peer);
+    const uint32_t peer_p_bar = ptx::MapToRank(bar(&misc->peer_p_full), peer);
+    Walk walk(p, misc);
+    Item item;
+    int lo, hi;
+    int g = 0;
+    int x = 0;  // exchanges with the peer
+    // Sends a value to the peer's thread of the same row and returns that thread's. Slots and barriers alternate: the peer
+    // sends its value of exchange x + 2 only after this thread's of x + 1, which this thread sends after it has read x.
+    auto exchange = [&](float v) -> float {
+      const int slot = x & 1;
+      const uint32_t mine = bar(&misc->max_full[slot][warp]);
+      if (lane == 0) ptx::MbarArriveExpectTx(mine, 32 * 4);
+      __syncwarp();
+      ptx::StAsyncF32(peer_max_at + slot * kRows * 4, v, peer_max_bar + slot * kSoftmaxWarps * 8);
+      if (!BoundedWait(mine, (x >> 1) & 1, misc, p.status, 33)) ok = false;
+      ++x;
+      return *reinterpret_cast<volatile float*>(&misc->peer_max[slot][row]);
+    };
+
+    while (ok && walk.Next(&item, &lo, &hi)) {
+      // Q's rows into tensor memory: T0, T1, V0-V3, 64 columns (32 registers) at a time. The item before this one has had its
+      // last S, so no MMA reads the old ones.
+      {
+        const int query = which == 0 ? item.q0 : item.q1;
+        const __nv_bfloat16* q_row = p.q + static_cast<int64_t>(query) * p.q_seq_stride + static_cast<int64_t>(head) * p.q_head_stride;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[3][32];
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const int slab = 3 * half + k;
+            const int at = 64 * (slab < 2 ? kVSlabs * (1 - rank) + slab : kVSlabs * rank + slab - 2);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              int4 w = make_int4(0, 0, 0, 0);
+              if (query >= 0) w = *reinterpret_cast<const int4*>(q_row + at + 8 * c);
+              v[k][4 * c] = w.x;
+              v[k][4 * c + 1] = w.y;
+              v[k][4 * c + 2] = w.z;
+              v[k][4 * c + 3] = w.w;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) ptx::TmemSt32(tmem + lane_base + kColQ + (3 * half + k) * 32, v[k]);
+        }
+        ptx::TmemWaitSt();
+        ptx::TcFenceBeforeSync();
+        __syncwarp();
+        if (lane == 0) ptx::MbarArrive(bar(&misc->qt_full));
+      }
+
+      float m_run = kLowest, l_run = 0.0f;
+      bool gave_up = false;
+      // The four warps leave this loop on the same vote (the named barriers have no bound): a wait that ran out goes on with
+      // whatever there is and asks for the rescaling path, where the vote is.
+      for (int s = lo; s < hi; ++s, ++g) {
+        const Step st = StepAt(item, s);
+        const int mine = max(0, min(kTile, st.valid - kTile * rank)), others = max(0, min(kTile, st.valid - kTile * static_cast<int>(peer)));
+        const int valid = (st.active >> which & 1) != 0 ? mine : 0;
+        if (!BoundedWait(bar(&misc->s_full), g & 1, misc, p.status, 30)) ok = false;
+        ptx::TcFenceAfterSync();
+        uint32_t sr[2][32];
+        ptx::TmemLd32(tmem + lane_base + kColS, sr[0]);
+        ptx::TmemLd32(tmem + lane_base + kColS + 32, sr[1]);
+        ptx::TmemWaitLd();
+        ptx::TcFenceBeforeSync();
+        __syncwarp();
+        if (lane == 0) ptx::MbarArrive(bar(&misc->s_empty));
+        float (&f)[2][32] = reinterpret_cast<float (&)[2][32]>(sr);
+        if (valid < kTile) {
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) {
+            if (c >= valid) f[c >> 5][c & 31] = -INFINITY;
+          }
+        }
+        float top[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) top[c] = f[0][c];
+#pragma unroll
+        for (int c = 8; c < kTile; ++c) top[c & 7] = fmaxf(top[c & 7], f[c >> 5][c & 31]);
+        float tile_max = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+        tile_max = fmaxf(tile_max, exchange(tile_max)) * p.scale_log2;
+        const bool moves = tile_max > m_run + kRescaleThreshold;
+        const bool rescale = moves && m_run != kLowest;
+        const float m_new = moves ? tile_max : m_run;
+        const float factor = rescale ? ptx::Ex2Approx(m_run - m_new) : 1.0f;
+        m_run = m_new;
+        l_run *= factor;
+        uint32_t packed[32];
+        float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float p0 = ptx::Ex2Approx(fmaf(f[c >> 4][2 * (c & 15)], p.scale_log2, -m_run));
+          const float p1 = ptx::Ex2Approx(fmaf(f[c >> 4][2 * (c & 15) + 1], p.scale_log2, -m_run));
+          const __nv_bfloat162 pb = __floats2bfloat162_rn(p0, p1);
+          packed[c] = *reinterpret_cast<const uint32_t*>(&pb);
+          part[c & 7] += p0 + p1;
+        }
+        l_run += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+
+        // The step before must be complete in both CTAs: its weights are overwritten, its sums scaled.
+        if (g > 0 && !BoundedWait(bar(&misc->pv_done), (g & 1) ^ 1, misc, p.status, 31)) ok = false;
+        if (ptx::NamedBarrierOr(1, kSoftmaxThreads, rescale || !ok)) {
+          misc->factor[row] = factor;
+          if (ptx::NamedBarrierOr(2, kSoftmaxThreads, !ok)) {
+            gave_up = true;
+            break;
+          }
+          ptx::TcFenceAfterSync();
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {  // columns of O^T are rows of S
+            uint32_t o[32];
+            ptx::TmemLd32(tmem + lane_base + kColO + 32 * c, o);
+            ptx::TmemWaitLd();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * misc->factor[32 * (c & 3) + k]);
+            ptx::TmemSt32(tmem + lane_base + kColO + 32 * c, o);
+          }
+          ptx::TmemWaitSt();
+          ptx::TcFenceBeforeSync();
+          ptx::NamedBarrier(2, kSoftmaxThreads);  // the factors have been read
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {  // 128-byte swizzle: chunk c of row r at c ^ (r % 8)
+          ptx::StShared128(p_row + ((c ^ (row & 7)) << 4), packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+        }
+        // Rows behind the end hold whatever the pool held there: zeroed, so that 0 x NaN cannot reach O. (A tile without any
+        // token was loaded as zeros.)
+        if (mine > 0 && mine < kTile) {
+          unsigned char* slabs = smem + kOffV + (g & 1) * kVSlabs * kSlabBytes;
+          for (int i = row; i < (kTile - mine) * kVSlabs * 8; i += kSoftmaxThreads) {
+            *reinterpret_cast<int4*>(slabs + ((i >> 3) & 3) * kSlabBytes + (mine + (i >> 5)) * 128 + (i & 7) * 16) = make_int4(0, 0, 0, 0);
+          }
+        }
+        if (others > 0 && others < kTile) {
+          if (!BoundedWait(bar(&misc->w_full[0]), g & 1, misc, p.status, 34) || !BoundedWait(bar(&misc->w_full[1]), g & 1, misc, p.status, 34)) ok = false;
+          for (int i = row; i < (kTile - others) * kVSlabs * 8; i += kSoftmaxThreads) {
+            *reinterpret_cast<int4*>(smem + kOffW + ((i >> 3) & 3) * kSlabBytes + (others + (i >> 5)) * 128 + (i & 7) * 16) = make_int4(0, 0, 0, 0);
+          }
+        }
+        ptx::FenceProxyAsync();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::BulkCopyToCta(peer_p_warp, p_warp, 32 * 128, peer_p_bar);
+          ptx::MbarArrive(bar(&misc->p_full));
+        }
+      }
+      if (gave_up) break;
+
+      // ---- epilogue of the item ----
+      const float l_all = l_run + exchange(l_run);
+      if (!BoundedWait(bar(&misc->pv_done), (g & 1) ^ 1, misc, p.status, 32)) ok = false;
+      ptx::TcFenceAfterSync();
+      const int n = item.steps();
+      const bool whole = lo == 0 && hi == n;
+      const int slot = 2 * run + (lo == 0 ? 1 : 0);
+      const int query = which == 0 ? item.q0 : item.q1;
+      misc->factor[row] = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+      if (rank == 0) {
+        if (row == 0) {
+          if (lo == 0) p.first_run[item.q0] = run;
+          if (hi == n) p.last_run[item.q0] = run;
+        }
+        if (!whole) {
+          p.ws_m[slot * kRows + row] = m_run;
+          p.ws_l[slot * kRows + row] = l_all;
+        } else if (p.lse != nullptr && query >= 0) {
+          p.lse[static_cast<int64_t>(query) * kHeads + head] =
+              l_all == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(m_run) * p.natural + static_cast<double>(logf(l_all)));
+        }
+      }
+      if (ptx::NamedBarrierOr(1, kSoftmaxThreads, !ok)) {
+        ok = false;
+        break;
+      }
+      const int queries = item.q1 >= 0 ? 2 : 1;
+#pragma unroll 1
+      for (int m = 0; m < 2; ++m) {
+        const int dv = kHalf * rank + 128 * m + row;
+#pragma unroll 1
+        for (int c = 0; c < 2 * queries; ++c) {  // 32 rows at a time
+          uint32_t o[32];
+          ptx::TmemLd32(tmem + lane_base + kColO + 128 * m + 32 * c, o);
+          ptx::TmemWaitLd();
+          if (!whole) {
+            uint4* dst = reinterpret_cast<uint4*>(p.ws_o) + (static_cast<int64_t>(slot) * (kRows / 4) + 8 * c) * kLatent + dv;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) dst[k * kLatent] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          } else {
+            __nv_bfloat16* dst = p.out + (static_cast<int64_t>(c < 2 ? item.q0 : item.q1) * kHeads + 32 * (c & 1)) * kLatent + dv;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float inv = misc->factor[32 * c + k];  // 0: no weights, and the accumulator may hold anything
+              dst[k * kLatent] = __float2bfloat16_rn(inv == 0.0f ? 0.0f : __uint_as_float(o[k]) * inv);
+            }
+          }
+        }
+      }
+      ptx::TcFenceBeforeSync();
+      ptx::NamedBarrier(2, kSoftmaxThreads);  // the factors have been read
+      if (lane == 0) ptx::MbarArrive(bar(&misc->o_empty));
+    }
+  }
+
+  // ---- teardown: the peer may still write into this CTA's shared memory until it has come here too ------------------
+  __syncthreads();
+  if (Aborting(misc)) {
+    // Copies may still be in flight towards this CTA or the peer (its weights, the tiles of an unfinished step): none takes
+    // longer than this.
+    const uint64_t t0 = ptx::GlobalTimerNs();
+    while (ptx::GlobalTimerNs() - t0 < 2000000ull) {
+    }
+  }
+  ptx::TcFenceBeforeSync();
+  ptx::ClusterArrive();
+  ptx::ClusterWait();
+  ptx::TcFenceAfterSync();
+  if (warp == 5) ptx::TmemDealloc(tmem, kTmemCols);
+}
+
+// Merges what the runs left of every item that was cut, and writes the result of queries without tokens. A CTA takes one query,
+// four of its heads and 256 / kGroups columns: a thread has one column of the four heads, 16 bytes a part, as the epilogue left
+// them. kGroups groups of threads share the parts out, so that the few queries of a long context have enough loads in flight.
+template <int kGroups>
+__global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constant__ SharedParams p) {
+  constexpr int kColumns = 256 / kGroups;
+  constexpr int kChunks = kLatent / kColumns;
+  constexpr int kBatch = 8;  // parts whose data a thread has in flight
+  const int query = blockIdx.x / (16 * kChunks);
+  const int quad = blockIdx.x / kChunks % 16;
+  const int dv = blockIdx.x % kChunks * kColumns + threadIdx.x % kColumns;
+  const int group = threadIdx.x / kColumns;
+  __shared__ float4 s_acc[kGroups > 1 ? 256 : 1];
+  GridDependencyWait();
+  GridDependencyTrigger();
+  const bool second = IsSecond(p.leader, query);
+  const int head = second ? query - 1 : query;  // the item's first query
+  __nv_bfloat16* out = p.out + (static_cast<int64_t>(query) * kHeads + 4 * quad) * kLatent + dv;
+  if (ItemAt(p, head).steps() == 0) {
+    if (group == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i * kLatent] = __float2bfloat16_rn(0.0f);
+      if (dv == 0 && p.lse != nullptr) {
+        for (int i = 0; i < 4; ++i) p.lse[static_cast<int64_t>(query) * kHeads + 4 * quad + i] = -INFINITY;
+      }
+    }
+    return;
+  }
+  const int first = p.first_run[head], last = p.last_run[head];
+  if (first >= last) return;  // one run held it all
+  const int row = (second ? kHeads : 0) + 4 * quad;
+  // Maxima and sums of the parts: part r is run first + r, whose slot is the one it begins in (r = 0) or continues in.
+  float m[4] = {kLowest, kLowest, kLowest, kLowest}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const uint4* ws = reinterpret_cast<const uint4*>(p.ws_o);
+  for (int r0 = first; r0 <= last; r0 += kBatch * kGroups) {
+    uint4 data[kBatch];
+    float4 pm[kBatch], pl[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = r0 + k * kGroups + group;
+      const bool there = r <= last && p.has_steps[r] != 0;
+      const int slot = 2 * r + (r == first ? 1 : 0);
+      pl[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      pm[k] = make_float4(kLowest, kLowest, kLowest, kLowest);
+      data[k] = make_uint4(0, 0, 0, 0);
+      if (there) {
+        pl[k] = *reinterpret_cast<const float4*>(p.ws_l + slot * kRows + row);
+        pm[k] = *reinterpret_cast<const float4*>(p.ws_m + slot * kRows + row);
+        data[k] = ws[(static_cast<int64_t>(slot) * (kRows / 4) + row / 4) * kLatent + dv];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float ml[4] = {pm[k].x, pm[k].y, pm[k].z, pm[k].w}, ll[4] = {pl[k].x, pl[k].y, pl[k].z, pl[k].w};
+      const uint32_t dd[4] = {data[k].x, data[k].y, data[k].z, data[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (ll[i] == 0.0f) continue;  // no weights, and the accumulator may hold anything (a NaN sum is not zero)
+        const float big = fmaxf(m[i], ml[i]);
+        const float w_old = exp2f(m[i] - big), w = exp2f(ml[i] - big);
+        acc[i] = acc[i] * w_old + __uint_as_float(dd[i]) * w;
+        l[i] = l[i] * w_old + ll[i] * w;
+        m[i] = big;
+      }
+    }
+  }
+  if constexpr (kGroups > 1) {
+    __shared__ float s_m[kGroups][4], s_l[kGroups][4];
+    s_acc[threadIdx.x] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (threadIdx.x % kColumns == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s_m[group][i] = m[i];
+        s_l[group][i] = l[i];
+      }
+    }
+    __syncthreads();
+    if (group != 0) return;
+    for (int o = 1; o < kGroups; ++o) {
+      const float4 other = s_acc[o * kColumns + threadIdx.x];
+      const float oa[4] = {other.x, other.y, other.z, other.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float ll = s_l[o][i], ml = s_m[o][i];
+        if (ll == 0.0f) continue;
+        const float big = fmaxf(m[i], ml);
+        const float w_old = exp2f(m[i] - big), w = exp2f(ml - big);
+        acc[i] = acc[i] * w_old + oa[i] * w;
+        l[i] = l[i] * w_old + ll * w;
+        m[i] = big;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i * kLatent] = __float2bfloat16_rn(l[i] == 0.0f ? 0.0f : acc[i] / l[i]);
+  if (dv == 0 && p.lse != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p.lse[static_cast<int64_t>(query) * kHeads + 4 * quad + i] =
+          l[i] == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(m[i]) * p.natural + static_cast<double>(logf(l[i])));
+    }
+  }
+}
+
+int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2; }
+
+size_t SharedWorkspaceBytes(int32_t batch) {
+  const size_t slots = static_cast<size_t>(RunsOfDevice()) * 2;
+  return slots * kRows * (kLatent + 2) * sizeof(float) + (2 * static_cast<size_t>(batch) + RunsOfDevice()) * 4 + 64;
+}
+
+bool SharedSupports(const b200kv_shared_args& a) {
+  return a.heads == kHeads && a.block_size % kTile == 0 && a.q_head_stride % 8 == 0 && a.q_seq_stride % 8 == 0 &&
+         (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && a.pool.pool_rows < INT32_MAX && a.pool.latent_row_stride * 2 < (1ll << 40);
+}
+
+int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* status) {
+  static thread_local int configured_device = -1;
+  int device = 0;
+  if (int32_t rc = CheckCuda(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+  if (device != configured_device) {
+    if (int32_t rc = CheckCuda(cudaFuncSetAttribute(MlaDecodeSharedKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes),
+                               "decode_shared smem opt-in")) {
+      return rc;
+    }
+    configured_device = device;
+  }
+  CUtensorMap latent_map, rope_map, q_map;
+  if (int32_t rc = GetRowMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, kLatent, kTile, &latent_map)) return rc;
+  if (int32_t rc = GetRowMap(a.pool.rope, a.pool.rope_row_stride, a.pool.pool_rows, kRope, kTile, &rope_map)) return rc;
+  if (int32_t rc = GetQMap(a.q, a.q_head_stride, a.q_seq_stride, a.batch, a.heads, kHeads, &q_map)) return rc;
+  const int32_t runs = RunsOfDevice();
+  SharedParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.q_seq_stride = a.q_seq_stride;
+  p.q_head_stride = a.q_head_stride;
+  p.block_table = a.block_table;
+  p.max_blocks = a.max_blocks;
+  p.table_rows = a.table_rows;
+  p.table_index = a.table_index;
+  p.kv_len = a.kv_len;
+  p.leader = a.leader;
+  p.shared_len = a.shared_len;
+  p.pool_rows = a.pool.pool_rows;
+  p.batch = a.batch;
+  p.block_size = a.block_size;
+  p.stable_tables = (a.flags & B200KV_DECODE_STABLE_TABLES) != 0 ? 1 : 0;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.natural = static_cast<double>(a.scale) / static_cast<double>(p.scale_log2);
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.lse = a.lse;
+  const size_t slots = static_cast<size_t>(runs) * 2;
+  p.ws_o = static_cast<float*>(a.workspace);
+  p.ws_m = p.ws_o + slots * kRows * kLatent;
+  p.ws_l = p.ws_m + slots * kRows;
+  p.first_run = reinterpret_cast<int32_t*>(p.ws_l + slots * kRows);
+  p.last_run = p.first_run + a.batch;
+  p.has_steps = p.last_run + a.batch;
+  p.status = status;
+  if (int32_t rc = CheckCuda(LaunchOverlapped(MlaDecodeSharedKernel, dim3(2 * static_cast<unsigned>(runs)), dim3(kThreads), kSmemBytes, stream,
+                                              latent_map, rope_map, q_map, p),
+                             "decode_shared launch")) {
+    return rc;
+  }
+  const unsigned quads = static_cast<unsigned>(a.batch) * 16;
+  const cudaError_t merged = a.batch <= 4 ? LaunchOverlapped(MlaSharedMergeKernel<4>, dim3(quads * 8), dim3(256), 0, stream, p)
+                                          : LaunchOverlapped(MlaSharedMergeKernel<1>, dim3(quads * 2), dim3(256), 0, stream, p);
+  return CheckCuda(merged, "decode_shared merge launch");
+}
+
+}  // namespace
+}  // namespace b200kv
+
+using namespace b200kv;
+
+extern "C" size_t b200kv_mla_decode_shared_workspace_bytes(int32_t batch, int32_t heads) {
+  if (batch <= 0 || heads <= 0) return 0;
+  const size_t own = SharedWorkspaceBytes(batch), plain = b200kv_mla_decode_workspace_bytes(batch, heads, 0);
+  return own > plain ? own : plain;
+}
+
+extern "C" int32_t b200kv_mla_decode_shared(const b200kv_shared_args* args, void* stream, b200kv_status_word* status) {
+  if (args == nullptr) {
+    SetLastError("decode_shared: args is null");
+    return B200KV_ERR_NULLPTR;
+  }
+  const b200kv_shared_args& a = *args;
+  if (int32_t rc = FaultCheck("b200kv_mla_decode_shared")) return rc;
+  if (int32_t rc = ValidatePoolView(&a.pool)) return rc;
+  if (a.batch == 0) return B200KV_OK;
+  if (a.q == nullptr || a.block_table == nullptr || a.kv_len == nullptr || a.leader == nullptr || a.shared_len == nullptr || a.out == nullptr) {
+    SetLastError("decode_shared: q, block_table, kv_len, leader, shared_len and out must be non-null");
+    return B200KV_ERR_NULLPTR;
+  }
+  if (a.batch < 0 || a.heads <= 0 || a.block_size <= 0 || a.max_blocks <= 0 || a.pool.pool_rows % a.block_size != 0 || !(a.scale > 0.0f) ||
+      a.q_head_stride < kLatent + kRope || (a.batch > 1 && a.q_seq_stride < 0) || (a.out_fp8 == nullptr) != (a.out_scale == nullptr) ||
+      a.table_rows < (a.table_index != nullptr ? 1 : a.batch)) {
+    SetLastError("decode_shared refused: batch %d heads %d block_size %d table %lld x %lld scale %g q strides %lld/%lld (a table row per query "
+                 "without table_index; out_fp8 and out_scale come together)",
+                 a.batch, a.heads, a.block_size, static_cast<long long>(a.table_rows), static_cast<long long>(a.max_blocks),
+                 static_cast<double>(a.scale), static_cast<long long>(a.q_seq_stride), static_cast<long long>(a.q_head_stride));
+    return B200KV_ERR_INVALID;
+  }
+  if (!SharedSupports(a)) {
+    // Any other geometry has each query read its own rows; the result is the same.
+    if (a.table_index != nullptr) {
+      SetLastError("decode_shared: table_index needs the tensor-core kernel's geometry (64 heads, block_size %% 64 == 0, 16-byte aligned q with "
+                   "strides that are multiples of 8 elements); heads %d, block_size %d", a.heads, a.block_size);
+      return B200KV_ERR_INVALID;
+    }
+    b200kv_decode_args d{};
+    d.q = a.q;
+    d.q_seq_stride = a.q_seq_stride;
+    d.q_head_stride = a.q_head_stride;
+    d.pool = a.pool;
+    d.block_table = a.block_table;
+    d.max_blocks = a.max_blocks;
+    d.kv_len = a.kv_len;
+    d.batch = a.batch;
+    d.heads = a.heads;
+    d.block_size = a.block_size;
+    d.scale = a.scale;
+    d.out = a.out;
+    d.lse = a.lse;
+    d.workspace = a.workspace;
+    d.workspace_bytes = a.workspace_bytes;
+    d.flags = a.flags;
+    d.out_fp8 = a.out_fp8;
+    d.out_scale = a.out_scale;
+    return b200kv_mla_decode(&d, stream, status);
+  }
+  const size_t need = SharedWorkspaceBytes(a.batch);
+  if (a.workspace == nullptr || a.workspace_bytes < need || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0) {
+    SetLastError("decode_shared: workspace of %zu bytes (16-byte aligned) required, %zu given", need, a.workspace_bytes);
+    return a.workspace == nullptr ? B200KV_ERR_NULLPTR : B200KV_ERR_INVALID;
+  }
+  if (int32_t rc = LaunchShared(a, static_cast<cudaStream_t>(stream), status)) return rc;
+  if (a.out_fp8 == nullptr) return B200KV_OK;
+  const int64_t cols = static_cast<int64_t>(a.heads) * kLatent;
+  return b200kv_mx_quant_e4m3(a.out, cols, a.batch, cols, a.out_fp8, cols, a.out_scale, cols / 32, stream);
+}

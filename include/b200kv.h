@@ -69,7 +69,7 @@ int32_t b200kv_abi_version(void);
  * FailRuntimeCall(name, calls) (mock/runtime_faults.cpp:8-23, used by tests/mock_failure_teardown.cpp:153-184).
  * Names: the device entry points b200kv_append, b200kv_gather, b200kv_resolve_rows, b200kv_mla_decode,
  * b200kv_mla_decode_peer, b200kv_lse_merge, b200kv_peer_merge, b200kv_append_fused, b200kv_mx_quant_e4m3,
- * b200kv_indexer_topk, and b200kv_engine_step_upload (the per-step copy of b200kv_engine_begin_step).
+ * b200kv_indexer_topk, b200kv_copy_blocks, b200kv_mla_decode_shared, and b200kv_engine_step_upload (the per-step copy of b200kv_engine_begin_step).
  * No GPU fault is ever made. b200kv_fault_clear disarms and returns how many injected failures fired.
  */
 int32_t b200kv_fault_inject(const char* entry_point, int32_t after_calls);
@@ -98,6 +98,18 @@ int32_t b200kv_gather(const b200kv_pool_view* pool, const int32_t* block_table, 
                       int64_t out_latent_stride, void* out_rope, int64_t out_rope_stride,
                       const int64_t* out_row_offsets, int64_t total_rows, void* stream,
                       b200kv_status_word* status);
+
+/*
+ * Pages copied inside the cache, in `layers` layers at once: for layer l and move i = (source block, destination block, rows), device
+ * int32 [n_moves][3], rows [0, rows) of the source block become those of the destination block, latent and rope. `pool` is
+ * layer 0's view; layer l lies latent_layer_stride and rope_layer_stride elements (multiples of 8) times l behind it. What
+ * b200kv_block_pool_fork, _unshare and _compact ask for. A move with a negative block, with rows 0 or onto itself is skipped; a
+ * block or row count out of range is recorded as B200KV_DEV_BAD_BLOCK (detail = move, value) and skipped. The moves are done in
+ * no order: no block may be the destination of two moves, nor the destination of one and the source of another. No counterpart
+ * in the reference, which keeps one sequence.
+ */
+int32_t b200kv_copy_blocks(const b200kv_pool_view* pool, int64_t layers, int64_t latent_layer_stride, int64_t rope_layer_stride,
+                           const int32_t* moves, int64_t n_moves, int64_t block_size, void* stream, b200kv_status_word* status);
 
 /*
  * Decode attention. Replaces the launch of aclnnFusedInferAttentionScoreV5 planned at
@@ -189,6 +201,49 @@ typedef struct b200kv_decode_args {
 
 size_t b200kv_mla_decode_workspace_bytes(int32_t batch, int32_t heads, int32_t max_ctas);
 int32_t b200kv_mla_decode(const b200kv_decode_args* args, void* stream, b200kv_status_word* status);
+
+/*
+ * Decode attention of queries that share rows of the cache: sequences forked from one prompt (b200kv_block_pool_fork), and
+ * several tokens of one sequence in a step (drafts to verify, a prompt's chunk), each of which attends up to itself. The result
+ * is that of b200kv_mla_decode with one table row per query; the shared rows are read once for two queries instead of once a
+ * query. No counterpart in the reference, which keeps one sequence and one token a step (src/memory/static_arena_manager.cpp:37-39).
+ * Query b attends over the first kv_len[b] tokens of table row table_index[b] (null: row b). leader and shared_len say what is
+ * shared: consecutive queries with the same leader[b] (the index of the first of them) form a group, and the table rows of a group
+ * name the same blocks for their first shared_len[b] tokens, which the kernel reads through any of the group's rows. The tokens of
+ * one sequence have one table_index and a shared_len of the longest kv_len, or more. A query that shares with nobody has
+ * leader[b] = b. kv_len 0 gives zeros and an lse of -infinity. All arrays device int32 of `batch` entries; block_table
+ * [table_rows][max_blocks], table_rows >= batch without table_index. A bad entry is recorded as B200KV_DEV_BAD_BLOCK (detail =
+ * query, column) and reads as zeros. Runs on tensor cores for 64 heads, block_size % 64 == 0 and a 16-byte aligned q with strides
+ * that are multiples of 8; any other geometry goes through b200kv_mla_decode (table_index is refused there). q, out, lse, scale,
+ * flags, out_fp8 and out_scale as in b200kv_decode_args; workspace of b200kv_mla_decode_shared_workspace_bytes() bytes.
+ */
+typedef struct b200kv_shared_args {
+  const void* q;
+  int64_t q_seq_stride;
+  int64_t q_head_stride;
+  b200kv_pool_view pool;
+  const int32_t* block_table;
+  int64_t max_blocks;
+  int64_t table_rows;
+  const int32_t* table_index; /* or null */
+  const int32_t* kv_len;
+  const int32_t* leader;
+  const int32_t* shared_len;
+  int32_t batch;
+  int32_t heads;
+  int32_t block_size;
+  float scale;
+  void* out;
+  float* lse; /* or null */
+  void* workspace;
+  size_t workspace_bytes;
+  uint32_t flags; /* B200KV_DECODE_STABLE_TABLES: leader, shared_len and table_index are meant too */
+  void* out_fp8;
+  void* out_scale;
+} b200kv_shared_args;
+
+size_t b200kv_mla_decode_shared_workspace_bytes(int32_t batch, int32_t heads);
+int32_t b200kv_mla_decode_shared(const b200kv_shared_args* args, void* stream, b200kv_status_word* status);
 
 /*
  * Attention over a selected subset of a sequence's tokens (what a top-k indexer in front of attention hands
