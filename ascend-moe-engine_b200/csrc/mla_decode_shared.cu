@@ -6,13 +6,13 @@
 //
 //   S   [128 rows x 64 tokens]    each CTA for ITS 64 of a step's 128 tokens:  Q (A) x K^T (B), M = 128 N = 64, 36 k-steps;
 //   P   = exp2(S * scale * log2e - m), bf16, written to shared memory and copied into the other CTA's;
-//   O^T [256 columns x 128 rows]  each CTA for ITS half of the 512 value columns, over all 128 tokens: V^T (A) x P^T (B),
-//                                 M = 128 N = 128, 2 x 8 k-steps.
+//   O   [128 rows x 256 columns]  each CTA for ITS half of the 512 value columns, over all 128 tokens: P (A) x V (B), M = 128
+//                                 N = 256, 8 k-steps.
 //
 // So each of the 128 x 512 sums lives in one CTA's tensor memory (a whole O would fill it and leave no room for S), nothing is
 // computed twice, every MMA has M = 128, and the tokens' rows that a CTA takes in are its own 64 x 576 and the other's
 // 64 x 256. Q does not fit beside them in shared memory: two thirds of it lie in tensor memory as the A operand, which also
-// halves what those MMAs read of shared memory. Tensor memory: O^T 256 columns, S 64, Q 192: all 512.
+// halves what those MMAs read of shared memory. Tensor memory: O 256 columns, S 64, Q 192: all 512.
 //
 // The two CTAs keep one running maximum: each sends its 128 rows' maxima over its tokens to the other before it exponentiates
 // (one asynchronous 4-byte store a thread), and both come to the same reference. As in the other kernels O is rescaled only when
@@ -21,7 +21,7 @@
 //
 // The list of work. A pair of queries is an item of n steps: first the tokens that both share (or a prefix of them: the tokens
 // of one sequence each attend up to themselves), then the first query's own tokens, then the second's, all into the same
-// accumulators; in the latter, only that query's 64 rows of P take part. All items' steps form one flat list, cut into one run
+// accumulators; in the latter, only that query's 64 lanes of O are touched. All items' steps form one flat list, cut into one run
 // per CTA pair by cost; a run's first and last item may be cut, and then leave fp32 partials (m, l, O) in the workspace which
 // the second kernel merges. A tile of tokens that is complete for one of the two queries only is two steps, one per query,
 // so that a NaN or an infinity in a row behind a query's end never meets that query's weights (0 x NaN).
@@ -38,6 +38,7 @@ namespace b200kv {
 
 int32_t ValidatePoolView(const b200kv_pool_view* pool);
 int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, CUtensorMap* out);
+int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, CUtensorMap* out);
 int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t box_heads,
                 CUtensorMap* out);
 
@@ -69,29 +70,44 @@ constexpr int kMiscBytes = 4096;
 constexpr int kSmemBytes = kOffMisc + kMiscBytes + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 
+struct Item {
+  int q0, q1;        // q1 < 0: a query alone
+  int len0, len1;
+  int lim0, lim1;    // tokens of the common part that each query attends over
+  int own;           // where the own tokens begin
+  int split;         // common tile that is two steps, or -1
+  int common, own0, own1;  // steps
+  __device__ __forceinline__ int steps() const { return common + own0 + own1; }
+};
+
+constexpr int kListed = 24;  // items of a run that the cut leaves in shared memory; a run of more walks the arrays again
+
 struct Misc {
   uint64_t t_full, t_empty;
-  // V and W come and go in halves of two slabs, the 128 columns of one accumulator: PV gives the first half back half way.
-  uint64_t v_full[2][2], v_empty[2][2];  // [set][half]
-  uint64_t w_full[2], w_empty[2];
+  uint64_t v_full[2], v_empty[2];
+  uint64_t w_full, w_empty;    // w_empty: PV of the step is complete
   uint64_t q_full, q_empty;    // the slabs in shared memory
   uint64_t qt_full;            // the slabs in tensor memory
   uint64_t s_full, s_empty;
   uint64_t p_full;             // own weights written, rows behind the end zeroed
   uint64_t peer_p_full;        // the other CTA's weights have landed
-  uint64_t pv_done;            // both CTAs' PV of a step are complete: the weights may be overwritten
+  uint64_t p_empty;            // PV has read this CTA's weights
+  uint64_t p_sent;             // and their copy has landed in the other CTA
+  uint64_t peer_p_empty;       // the other CTA's PV has read the copy it holds of them
   uint64_t o_empty;
   uint64_t max_full[2][kSoftmaxWarps];
   uint64_t drain[2];
   uint32_t tmem_base;
   int32_t abort_flag;
-  int32_t start_query;  // the run's first item, the step in it, and how many steps
+  int32_t start_query;  // the run's first item, its ordinal, the step in it, the run that it began in
   int32_t start_step;
-  int32_t n_steps;
-  unsigned long long flat_lo, flat_hi;
-  unsigned long long scan[8][2];
+  int32_t began_in;
+  int32_t n_items;
+  long long start_ordinal, end_ordinal;
+  long long flat_lo, flat_hi;
+  long long scan[8][3];
   float peer_max[2][kRows];
-  float factor[kRows];
+  Item items[kListed];  // by ordinal % kListed
 };
 static_assert(sizeof(Misc) <= kMiscBytes, "Misc does not fit its reservation");
 
@@ -114,14 +130,12 @@ struct SharedParams {
   double natural;  // scale / scale_log2: from the kernels' log2 domain back to natural logarithms
   __nv_bfloat16* out;
   float* lse;
-  // Partials: slot 2c of run c is an item it continues, slot 2c + 1 one it begins and does not finish. O as [slot][32 row
-  // quads][512 columns][4 rows]: an epilogue thread owns a column and has its rows in consecutive registers.
-  float* ws_o;
+  // Partials: slot 2c of run c is an item it continues, slot 2c + 1 one it begins and does not finish. O as [slot][128 column
+  // quads][128 rows][4 columns]: an epilogue thread owns a row, and a warp's stores are 512 contiguous bytes.
+  float4* ws_o;
   float* ws_m;  // [slot][128], log2 domain
   float* ws_l;
-  int32_t* first_run;  // [batch], by an item's first query: the runs that hold its first and its last step
-  int32_t* last_run;
-  int32_t* has_steps;  // [runs]
+  int4* merges;  // [runs]: the item that run c finishes and another began: its queries, the run that began it; x < 0: none
   int32_t* status;
 };
 
@@ -131,16 +145,6 @@ struct SharedParams {
 __device__ __forceinline__ bool IsSecond(const int32_t* leader, int b) {
   return b > 0 && leader[b] == leader[b - 1] && ((static_cast<unsigned>(b - 1) - static_cast<unsigned>(leader[b - 1])) & 1u) == 0;
 }
-
-struct Item {
-  int q0, q1;        // q1 < 0: a query alone
-  int len0, len1;
-  int lim0, lim1;    // tokens of the common part that each query attends over
-  int own;           // where the own tokens begin
-  int split;         // common tile that is two steps, or -1
-  int common, own0, own1;  // steps
-  __device__ __forceinline__ int steps() const { return common + own0 + own1; }
-};
 
 __device__ __forceinline__ int StepsOf(int tokens) { return tokens > 0 ? (tokens - 1) / kStep + 1 : 0; }
 
@@ -227,38 +231,42 @@ struct Cut {
 // The items of this run, one after the other. Every role runs the same walk.
 struct Walk {
   const SharedParams& p;
-  int query;
+  const Misc* misc;
+  int at;         // item of the run, or query where the run has too many to be listed
   int step;
-  int remaining;
-  __device__ Walk(const SharedParams& params, const Misc* misc)
-      : p(params), query(misc->start_query), step(misc->start_step), remaining(misc->n_steps) {}
+  long long remaining;
+  bool listed;
+  __device__ Walk(const SharedParams& params, const Misc* m)
+      : p(params), misc(m), step(m->start_step), remaining(m->flat_hi - m->flat_lo), listed(m->n_items <= kListed) {
+    at = listed ? 0 : m->start_query;
+  }
   __device__ bool Next(Item* item, int* lo, int* hi) {
-    while (remaining > 0 && query < p.batch) {
-      if (!IsSecond(p.leader, query)) {
-        const Item it = ItemAt(p, query);
-        const int n = it.steps();
-        if (step < n) {
-          const int take = min(remaining, n - step);
-          *item = it;
-          *lo = step;
-          *hi = step + take;
-          remaining -= take;
-          step = 0;
-          ++query;  // (an item that is not finished here is the run's last)
-          return true;
-        }
+    if (remaining <= 0) return false;
+    if (listed) {
+      *item = misc->items[(misc->start_ordinal + at) % kListed];
+      ++at;
+    } else {
+      for (;; ++at) {
+        if (at >= p.batch) return false;
+        if (IsSecond(p.leader, at)) continue;
+        *item = ItemAt(p, at);
+        if (item->steps() > 0) break;
       }
-      step = 0;
-      ++query;
+      ++at;  // (an item that is not finished here is the run's last)
     }
-    return false;
+    *lo = step;
+    *hi = static_cast<int>(min(remaining, static_cast<long long>(item->steps() - step))) + step;
+    remaining -= *hi - step;
+    step = 0;
+    return true;
   }
 };
 
-// A bounded wait by all lanes of a warp together, behind an inline probe.
+// A bounded wait by all lanes of a warp together, behind an inline probe. It spins: a parked warp resumes some 500 cycles after
+// its phase, a fifth of a step.
 __device__ __forceinline__ bool WarpWait(uint32_t bar, uint32_t parity, Misc* misc, int32_t* status, int site) {
   if (__all_sync(0xffffffffu, ptx::MbarTestWait(bar, parity))) return true;
-  return __all_sync(0xffffffffu, BoundedWait(bar, parity, misc, status, site));
+  return __all_sync(0xffffffffu, BoundedSpin(bar, parity, misc, status, site));
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -280,15 +288,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::MbarInit(bar(&misc->t_full), 1);
     ptx::MbarInit(bar(&misc->t_empty), 1);
     for (int s = 0; s < 2; ++s) {
-      for (int h = 0; h < 2; ++h) {
-        ptx::MbarInit(bar(&misc->v_full[s][h]), 1);
-        ptx::MbarInit(bar(&misc->v_empty[s][h]), 1);
-      }
-      ptx::MbarInit(bar(&misc->w_full[s]), 1);
-      ptx::MbarInit(bar(&misc->w_empty[s]), 1);
+      ptx::MbarInit(bar(&misc->v_full[s]), 1);
+      ptx::MbarInit(bar(&misc->v_empty[s]), 1);
       ptx::MbarInit(bar(&misc->drain[s]), 1);
       for (int w = 0; w < kSoftmaxWarps; ++w) ptx::MbarInit(bar(&misc->max_full[s][w]), 1);
     }
+    ptx::MbarInit(bar(&misc->w_full), 1);
+    ptx::MbarInit(bar(&misc->w_empty), 1);
     ptx::MbarInit(bar(&misc->q_full), 1);
     ptx::MbarInit(bar(&misc->q_empty), 1);
     ptx::MbarInit(bar(&misc->qt_full), kSoftmaxWarps);
@@ -296,12 +302,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::MbarInit(bar(&misc->s_empty), kSoftmaxWarps);
     ptx::MbarInit(bar(&misc->p_full), kSoftmaxWarps);
     ptx::MbarInit(bar(&misc->peer_p_full), 1);
-    ptx::MbarInit(bar(&misc->pv_done), 2);
+    ptx::MbarInit(bar(&misc->p_empty), 1);
+    ptx::MbarInit(bar(&misc->p_sent), 1);
+    ptx::MbarInit(bar(&misc->peer_p_empty), 1);
     ptx::MbarInit(bar(&misc->o_empty), kSoftmaxWarps);
     misc->abort_flag = 0;
     misc->start_query = p.batch;
     misc->start_step = 0;
-    misc->n_steps = 0;
+    misc->began_in = 0;
+    misc->start_ordinal = misc->end_ordinal = 0;
     ptx::FenceBarrierInit();
     ptx::PrefetchTensorMap(&latent_map);
     ptx::PrefetchTensorMap(&rope_map);
@@ -317,40 +326,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // (let go only after this kernel's own wait: the merge kernel reads the lengths too)
 
   // ---- this run of the list: totals, then the first step at or after the run's first cost position and the next run's ------
+  long long empty = 0;  // items without steps
+  int runs_used;
   {
-    unsigned long long steps = 0, items = 0;
+    long long steps = 0, items = 0;
+    Item mine;
+    int mine_n = 0;  // the first chunk's item of this thread, kept
     for (int b = threadIdx.x; b < p.batch; b += kThreads) {
-      const int n = IsSecond(p.leader, b) ? 0 : ItemAt(p, b).steps();
+      if (IsSecond(p.leader, b)) continue;
+      const Item it = ItemAt(p, b);
+      const int n = it.steps();
+      if (b < kThreads) {
+        mine = it;
+        mine_n = n;
+      }
       steps += n;
       items += n > 0 ? 1 : 0;
+      empty += n > 0 ? 0 : 1;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
       steps += __shfl_xor_sync(0xffffffffu, steps, off);
       items += __shfl_xor_sync(0xffffffffu, items, off);
+      empty += __shfl_xor_sync(0xffffffffu, empty, off);
     }
     if (lane == 0) {
       misc->scan[warp][0] = steps;
       misc->scan[warp][1] = items;
+      misc->scan[warp][2] = empty;
     }
     __syncthreads();
     long long total = 0, total_items = 0;
+    empty = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
       total += misc->scan[w][0];
       total_items += misc->scan[w][1];
+      empty += misc->scan[w][2];
     }
     if (threadIdx.x == 0) {
       misc->flat_lo = total;
       misc->flat_hi = total;
     }
-    const Cut cut{Cut::Pos(total, total_items > 0 ? total_items - 1 : 0), runs};
+    const long long cost = Cut::Pos(total, total_items > 0 ? total_items - 1 : 0);
+    // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty.
+    runs_used = static_cast<int>(min(static_cast<long long>(runs), max(1ll, cost / Cut::kStepCost)));
+    const Cut cut{cost, runs_used};
     const long long k_lo = cut.First(run), k_hi = cut.First(run + 1);
     long long before = 0, before_items = 0;
     for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
       __syncthreads();
       const int b = b0 + threadIdx.x;
-      const int n = b < p.batch && !IsSecond(p.leader, b) ? ItemAt(p, b).steps() : 0;
+      if (b0 > 0) {
+        mine_n = 0;
+        if (b < p.batch && !IsSecond(p.leader, b)) {
+          mine = ItemAt(p, b);
+          mine_n = mine.steps();
+        }
+      }
+      const int n = mine_n;
       long long incl = n, incl_items = n > 0 ? 1 : 0;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -376,19 +410,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         chunk += misc->scan[w][0];
         chunk_items += misc->scan[w][1];
       }
-      if (n > 0) {
+      if (n > 0 && run < runs_used) {
         const long long first = before + incl - n, s = before_items + incl_items - 1;
-        const long long last_pos = Cut::Pos(first + n - 1, s);
+        const long long first_pos = Cut::Pos(first, s), last_pos = Cut::Pos(first + n - 1, s);
         const long long last_before = Cut::Pos(first - 1, s - 1);  // the item before this one ends here
         auto at_or_after = [&](long long k) {                      // first step at or after cost position k, if it is in this item
           const long long x = (k - Cut::kEnterCost * s + 1) >> 1;
           return x > first ? x : first;
         };
-        if (last_pos >= k_lo && (s == 0 || last_before < k_lo)) {
-          const long long x = at_or_after(k_lo);
-          misc->flat_lo = x;
-          misc->start_query = b;
-          misc->start_step = static_cast<int>(x - first);
+        if (last_pos >= k_lo && first_pos < k_hi) {
+          misc->items[s % kListed] = mine;  // (more than kListed overwrite each other and are not read)
+          if (s == 0 || last_before < k_lo) {
+            const long long x = at_or_after(k_lo);
+            misc->flat_lo = x;
+            misc->start_query = b;
+            misc->start_step = static_cast<int>(x - first);
+            misc->start_ordinal = s;
+            misc->began_in = static_cast<int>(first_pos * runs_used / cost);
+          }
+          atomicMax(reinterpret_cast<unsigned long long*>(&misc->end_ordinal), static_cast<unsigned long long>(s + 1));
         }
         if (last_pos >= k_hi && (s == 0 || last_before < k_hi)) misc->flat_hi = at_or_after(k_hi);
       }
@@ -399,12 +439,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::TcFenceBeforeSync();
   __syncthreads();
   ptx::TcFenceAfterSync();
-  if (threadIdx.x == 0) misc->n_steps = static_cast<int>(misc->flat_hi - misc->flat_lo);
+  if (threadIdx.x == 0) misc->n_items = static_cast<int>(min(misc->end_ordinal - misc->start_ordinal, 1ll << 30));
   if (p.stable_tables != 0) GridDependencyWait();
   GridDependencyTrigger();
   __syncthreads();
   ptx::ClusterWait();
-  if (threadIdx.x == 0 && rank == 0) p.has_steps[run] = misc->n_steps > 0 ? 1 : 0;
+  if (threadIdx.x == 0 && rank == 0) p.merges[run] = make_int4(-1, -1, 0, 0);
+  if (empty > 0) {  // queries that attend over nothing, alone or with one like them
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      const int first = IsSecond(p.leader, b) ? b - 1 : b;
+      if (ItemAt(p, first).steps() > 0) continue;
+      int4* out = reinterpret_cast<int4*>(p.out + static_cast<int64_t>(b) * kHeads * kLatent);
+      for (int i = threadIdx.x; i < kHeads * kLatent / 8; i += kThreads) out[i] = make_int4(0, 0, 0, 0);
+      if (p.lse != nullptr && threadIdx.x < kHeads) p.lse[static_cast<int64_t>(b) * kHeads + threadIdx.x] = -INFINITY;
+    }
+  }
 
   const uint32_t tmem = misc->tmem_base;
   bool ok = true;
@@ -430,15 +479,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       return static_cast<int32_t>(row);
     };
-    // Warp 4, lane l < 5: slab T(l); l < 9: V(l - 5). Warp 7, lane l < 4: the other tile's slab of the same columns as V(l).
-    const bool is_w = warp == 7, is_t = !is_w && lane < kTSlabs;
-    const bool loader = lane < (is_w ? kVSlabs : kTSlabs + kVSlabs);
-    const int j = is_t || is_w ? lane : lane - kTSlabs;
-    const int column = 64 * (is_t ? kVSlabs * (1 - rank) + j : kVSlabs * rank + j);  // (T4 is the rope slab)
-    const bool announces = is_t ? j == 0 : (j & 1) == 0;
-    const uint32_t announced = (is_t ? kTSlabs : 2) * kSlabBytes;
-    const int half = is_t ? 0 : (j >> 1) & 1;
-    const uint32_t dst0 = base + (is_t ? kOffT : is_w ? kOffW : kOffV) + j * kSlabBytes;
+    // Warp 4: lane 0 T's four latent slabs, lane 1 its rope slab, lane 2 V. Warp 7: lane 0 the other tile's slabs of V's columns.
+    // Four slabs are one box: a warp issues a load only every 170 cycles or so.
+    const bool is_w = warp == 7, is_t = !is_w && lane < 2;
+    const bool loader = lane < (is_w ? 1 : 3);
+    const bool is_rope = is_t && lane == 1;
+    const int first_slab = is_t ? kVSlabs * (1 - rank) : kVSlabs * rank;
+    const bool announces = loader && !is_rope;
+    const uint32_t announced = (is_t ? kTSlabs : kVSlabs) * kSlabBytes;
+    const uint32_t dst0 = base + (is_t ? kOffT : is_w ? kOffW : kOffV) + (is_rope ? kVSlabs * kSlabBytes : 0);
     Walk walk(p, misc);
     Item item;
     int lo, hi;
@@ -462,8 +511,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int s = lo; s < hi; ++s, ++g) {
         const int32_t row = tile_row(StepAt(item, s), is_w ? 1 - rank : rank);
         const int set = g & 1;
-        const uint32_t full = is_t ? bar(&misc->t_full) : is_w ? bar(&misc->w_full[half]) : bar(&misc->v_full[set][half]);
-        const uint32_t empty = is_t ? bar(&misc->t_empty) : is_w ? bar(&misc->w_empty[half]) : bar(&misc->v_empty[set][half]);
+        const uint32_t full = is_t ? bar(&misc->t_full) : is_w ? bar(&misc->w_full) : bar(&misc->v_full[set]);
+        const uint32_t empty = is_t ? bar(&misc->t_empty) : is_w ? bar(&misc->w_empty) : bar(&misc->v_empty[set]);
         const uint32_t dst = dst0 + (!is_t && !is_w ? set * kVSlabs * kSlabBytes : 0);
         // Phase of the buffer's last use: T and W are used every step, a V set every other.
         const bool every = is_t || is_w;
@@ -475,10 +524,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (uint32_t it = 0;; ++it) {
           if (!done && (first_use || ptx::MbarTestWait(empty, parity))) {
             if (announces) ptx::MbarArriveExpectTx(full, announced);
-            if (is_t && j == kTSlabs - 1) {
+            if (is_rope) {
               ptx::TmaLoad2D(dst, &rope_map, 0, row, full);
             } else {
-              ptx::TmaLoad2D(dst, &latent_map, column, row, full);
+              ptx::TmaLoad3D(dst, &latent_map, 0, row, first_slab, full);
             }
             done = true;
           }
@@ -536,20 +585,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty));
         const int set = __shfl_sync(0xffffffffu, g & 1, 0);
         const uint64_t v_desc = DescAt(v_desc0, set * kVSlabs * kSlabBytes);
+        ok = WarpWait(bar(&misc->v_full[set]), (g >> 1) & 1, misc, p.status, 26);
+        if (!ok) break;
+        ptx::TcFenceAfterSync();
 #pragma unroll
-        for (int half = 0; half < 2 && ok; ++half) {
-          ok = WarpWait(bar(&misc->v_full[set][half]), (g >> 1) & 1, misc, p.status, 26);
-          if (!ok) break;
-          ptx::TcFenceAfterSync();
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int slab = 2 * half + (k >> 2), kk = k & 3;
-            if (ptx::ElectOne()) {
-              ptx::MmaF16TS(d, tmem_u + kColQ + (2 + slab) * 32 + kk * 8, DescAt(v_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
-            }
+        for (int k = 0; k < 4 * kVSlabs; ++k) {
+          const int slab = k >> 2, kk = k & 3;
+          if (ptx::ElectOne()) {
+            ptx::MmaF16TS(d, tmem_u + kColQ + (2 + slab) * 32 + kk * 8, DescAt(v_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
           }
         }
-        if (!ok) break;
         if (ptx::ElectOne()) {
           ptx::TcCommit(bar(&misc->s_full));
           if (i == n - 1) ptx::TcCommit(bar(&misc->q_empty));
@@ -567,12 +612,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 6) {
     // ======================= PV ================================================================================
-    constexpr uint32_t kIdescBoth = ptx::InstrDescBf16(128, kRows, 1, 0);
-    constexpr uint32_t kIdescOne = ptx::InstrDescBf16(128, kHeads, 1, 0);
+    constexpr uint32_t kIdesc = ptx::InstrDescBf16(kRows, kHalf, 0, 1);
     const uint64_t p_desc = ptx::SmemDescSw128(base + kOffP, 16, 1024);  // K-major: row = row of P, 32 bytes a k-step
     const uint64_t peer_p_desc = DescAt(p_desc, kOffPeerP - kOffP);
-    const uint64_t v_desc0 = ptx::SmemDescSw128(base + kOffV, kSlabBytes, 1024);  // MN-major: next 64 columns a slab further
+    const uint64_t v_desc0 = ptx::SmemDescSw128(base + kOffV, kSlabBytes, 1024);  // MN-major B: next 64 columns a slab further
     const uint64_t w_desc = DescAt(v_desc0, kOffW - kOffV);
+    const uint32_t peer_p_sent = ptx::MapToRank(bar(&misc->p_sent), rank ^ 1);
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
     Walk walk(p, misc);
     Item item;
@@ -586,35 +631,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int s = lo; s < hi && ok; ++s, ++g) {
         const int active = __shfl_sync(0xffffffffu, StepAt(item, s).active, 0);
         if (ptx::ElectOne()) ptx::MbarArriveExpectTx(bar(&misc->peer_p_full), kPBytes);
-        ok = WarpWait(bar(&misc->w_full[0]), g & 1, misc, p.status, 28) && WarpWait(bar(&misc->w_full[1]), g & 1, misc, p.status, 28) &&
-             WarpWait(bar(&misc->p_full), g & 1, misc, p.status, 21) && WarpWait(bar(&misc->peer_p_full), g & 1, misc, p.status, 29);
+        ok = WarpWait(bar(&misc->p_full), g & 1, misc, p.status, 21);
         if (!ok) break;
         ptx::TcFenceAfterSync();
         const int set = __shfl_sync(0xffffffffu, g & 1, 0);
         const uint64_t v_desc = DescAt(v_desc0, set * kVSlabs * kSlabBytes);
-        // Both queries' rows in one pass, or (one of them takes no part, or has begun and the other has not) a pass of 64.
+        // Both queries' rows in one pass, or (one of them takes no part, or has begun and the other has not) a pass for each that
+        // leaves the other's lanes alone. This CTA's tokens first: the other's weights are on their way meanwhile.
         const bool one_pass = active == 3 && (started == 0 || started == 3);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          for (int pass = 0; pass < 2; ++pass) {
-            if (one_pass ? pass == 1 : (active >> pass & 1) == 0) continue;
-            const uint32_t idesc = one_pass ? kIdescBoth : kIdescOne;
-            const uint32_t at = one_pass ? 0 : pass * kHeads;  // first row
-            const uint32_t keep = (started >> pass) & 1;
-            const uint64_t pd = DescAt(p_desc, at * 128), ppd = DescAt(peer_p_desc, at * 128);
+        for (int theirs = 0; theirs < 2; ++theirs) {
+          if (theirs != 0) {
+            ok = WarpWait(bar(&misc->peer_p_full), g & 1, misc, p.status, 29);
+            if (!ok) break;
+            if (ptx::ElectOne()) ptx::MbarArriveRemote(peer_p_sent);
+            ok = WarpWait(bar(&misc->w_full), g & 1, misc, p.status, 28);
+            if (!ok) break;
+            ptx::TcFenceAfterSync();
+          }
+          const uint64_t weights = theirs != 0 ? peer_p_desc : p_desc, values = theirs != 0 ? w_desc : v_desc;
+          if (one_pass) {
+            const uint32_t keep = theirs != 0 || started != 0 ? 1u : 0u;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {  // four k-steps of this CTA's tokens, four of the other's
-              const uint64_t a = DescAt(k < 4 ? v_desc : w_desc, 2 * m * kSlabBytes + (k & 3) * 2048);
-              const uint64_t b = DescAt(k < 4 ? pd : ppd, (k & 3) * 32);
-              if (ptx::ElectOne()) ptx::MmaF16SS(tmem_u + kColO + 128 * m + at, a, b, idesc, k > 0 ? 1u : keep);
+            for (int k = 0; k < kTile / 16; ++k) {
+              if (ptx::ElectOne()) ptx::MmaF16SS(tmem_u + kColO, DescAt(weights, k * 32), DescAt(values, k * 2048), kIdesc, k > 0 ? 1u : keep);
+            }
+          } else {
+            for (int q = 0; q < 2; ++q) {
+              if ((active >> q & 1) == 0) continue;
+              const uint32_t keep = theirs != 0 ? 1u : (started >> q) & 1;
+              const uint32_t off_lo = q == 0 ? 0u : 0xffffffffu;
+#pragma unroll
+              for (int k = 0; k < kTile / 16; ++k) {
+                if (ptx::ElectOne()) {
+                  ptx::MmaF16SSLanes(tmem_u + kColO, DescAt(weights, k * 32), DescAt(values, k * 2048), kIdesc, off_lo, ~off_lo, k > 0 ? 1u : keep);
+                }
+              }
             }
           }
           if (ptx::ElectOne()) {
-            if (m == 1) ptx::TcCommitTo(bar(&misc->pv_done), 3);
-            ptx::TcCommit(bar(&misc->v_empty[set][m]));
-            ptx::TcCommit(bar(&misc->w_empty[m]));
+            if (theirs == 0) {
+              ptx::TcCommit(bar(&misc->v_empty[set]));
+              ptx::TcCommit(bar(&misc->p_empty));
+            } else {
+              ptx::TcCommit(bar(&misc->w_empty));
+              ptx::TcCommitTo(bar(&misc->peer_p_empty), static_cast<uint16_t>(1u << (rank ^ 1)));
+            }
           }
         }
+        if (!ok) break;
         started |= active;
       }
       ++seg;
@@ -652,52 +717,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (lane == 0) ptx::MbarArriveExpectTx(mine, 32 * 4);
       __syncwarp();
       ptx::StAsyncF32(peer_max_at + slot * kRows * 4, v, peer_max_bar + slot * kSoftmaxWarps * 8);
-      if (!BoundedWait(mine, (x >> 1) & 1, misc, p.status, 33)) ok = false;
+      ok = WarpWait(mine, (x >> 1) & 1, misc, p.status, 33) && ok;
       ++x;
       return *reinterpret_cast<volatile float*>(&misc->peer_max[slot][row]);
     };
-
-    while (ok && walk.Next(&item, &lo, &hi)) {
-      // Q's rows into tensor memory: T0, T1, V0-V3, 64 columns (32 registers) at a time. The item before this one has had its
-      // last S, so no MMA reads the old ones.
-      {
-        const int query = which == 0 ? item.q0 : item.q1;
-        const __nv_bfloat16* q_row = p.q + static_cast<int64_t>(query) * p.q_seq_stride + static_cast<int64_t>(head) * p.q_head_stride;
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          uint32_t v[3][32];
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const int slab = 3 * half + k;
-            const int at = 64 * (slab < 2 ? kVSlabs * (1 - rank) + slab : kVSlabs * rank + slab - 2);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              int4 w = make_int4(0, 0, 0, 0);
-              if (query >= 0) w = *reinterpret_cast<const int4*>(q_row + at + 8 * c);
-              v[k][4 * c] = w.x;
-              v[k][4 * c + 1] = w.y;
-              v[k][4 * c + 2] = w.z;
-              v[k][4 * c + 3] = w.w;
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 3; ++k) ptx::TmemSt32(tmem + lane_base + kColQ + (3 * half + k) * 32, v[k]);
-        }
-        ptx::TmemWaitSt();
-        ptx::TcFenceBeforeSync();
-        __syncwarp();
-        if (lane == 0) ptx::MbarArrive(bar(&misc->qt_full));
+    // The warp's weights of step g - 1 may be overwritten: PV has read them, and so has the copy.
+    auto weights_free = [&]() {
+      if (g > 0) {
+        ok = WarpWait(bar(&misc->p_empty), (g & 1) ^ 1, misc, p.status, 31) && WarpWait(bar(&misc->p_sent), (g & 1) ^ 1, misc, p.status, 38) && ok;
       }
-
+    };
+    // An item's rows of Q into tensor memory: T0, T1, V0-V3. A row is a lane there, and a warp reads four rows' 128 bytes with one
+    // instruction, so they change places in the warp's part of the weights' buffer. The item before has had its last S, so no MMA
+    // reads the old ones.
+    auto load_q = [&](const Item& it) {
+      const int query = which == 0 ? it.q0 : it.q1;  // (the same for the whole warp)
+      const int sub = lane >> 3, chunk = lane & 7;
+      const __nv_bfloat16* q_rows = p.q + static_cast<int64_t>(query) * p.q_seq_stride + static_cast<int64_t>((warp & 1) * 32 + sub) * p.q_head_stride + 8 * chunk;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        int4 v[3][8];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const int slab = 3 * half + k;
+          const int at = 64 * (slab < 2 ? kVSlabs * (1 - rank) + slab : kVSlabs * rank + slab - 2);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[k][i] = make_int4(0, 0, 0, 0);
+            if (query >= 0) v[k][i] = *reinterpret_cast<const int4*>(q_rows + static_cast<int64_t>(4 * i) * p.q_head_stride + at);
+          }
+        }
+        if (half == 0) weights_free();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // row 4 i + sub of the warp's 32
+            ptx::StShared128(p_warp + (4 * i + sub) * 128 + ((chunk ^ (4 * (i & 1) + sub)) << 4), v[k][i].x, v[k][i].y, v[k][i].z, v[k][i].w);
+          }
+          __syncwarp();
+          uint32_t r[32];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) ptx::LdShared128(p_row + ((c ^ (row & 7)) << 4), r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+          ptx::TmemSt32(tmem + lane_base + kColQ + (3 * half + k) * 32, r);
+        }
+      }
+      ptx::TmemWaitSt();
+      ptx::TcFenceBeforeSync();
+      __syncwarp();
+      if (lane == 0) ptx::MbarArrive(bar(&misc->qt_full));
+    };
+    Item next_item;
+    int next_lo = 0, next_hi = 0;
+    bool more = walk.Next(&next_item, &next_lo, &next_hi);
+    bool continued = misc->start_step > 0;
+    if (more) load_q(next_item);
+    while (ok && more) {
+      item = next_item;
+      lo = next_lo;
+      hi = next_hi;
       float m_run = kLowest, l_run = 0.0f;
-      bool gave_up = false;
-      // The four warps leave this loop on the same vote (the named barriers have no bound): a wait that ran out goes on with
-      // whatever there is and asks for the rescaling path, where the vote is.
-      for (int s = lo; s < hi; ++s, ++g) {
+      for (int s = lo; s < hi && ok; ++s, ++g) {  // (ok is the warp's; warps that give up leave the others' waits to run out)
         const Step st = StepAt(item, s);
         const int mine = max(0, min(kTile, st.valid - kTile * rank)), others = max(0, min(kTile, st.valid - kTile * static_cast<int>(peer)));
         const int valid = (st.active >> which & 1) != 0 ? mine : 0;
-        if (!BoundedWait(bar(&misc->s_full), g & 1, misc, p.status, 30)) ok = false;
+        ok = WarpWait(bar(&misc->s_full), g & 1, misc, p.status, 30) && ok;
         ptx::TcFenceAfterSync();
         uint32_t sr[2][32];
         ptx::TmemLd32(tmem + lane_base + kColS, sr[0]);
@@ -738,27 +822,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         l_run += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
 
-        // The step before must be complete in both CTAs: its weights are overwritten, its sums scaled.
-        if (g > 0 && !BoundedWait(bar(&misc->pv_done), (g & 1) ^ 1, misc, p.status, 31)) ok = false;
-        if (ptx::NamedBarrierOr(1, kSoftmaxThreads, rescale || !ok)) {
-          misc->factor[row] = factor;
-          if (ptx::NamedBarrierOr(2, kSoftmaxThreads, !ok)) {
-            gave_up = true;
-            break;
-          }
+        weights_free();
+        if (__any_sync(0xffffffffu, rescale)) {
+          // The warp's lanes of O are scaled between this step's PV and the one before.
+          if (g > 0) ok = WarpWait(bar(&misc->w_empty), (g & 1) ^ 1, misc, p.status, 35) && ok;
           ptx::TcFenceAfterSync();
 #pragma unroll 1
-          for (int c = 0; c < 8; ++c) {  // columns of O^T are rows of S
+          for (int c = 0; c < kHalf / 32; ++c) {
             uint32_t o[32];
             ptx::TmemLd32(tmem + lane_base + kColO + 32 * c, o);
             ptx::TmemWaitLd();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * misc->factor[32 * (c & 3) + k]);
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
             ptx::TmemSt32(tmem + lane_base + kColO + 32 * c, o);
           }
           ptx::TmemWaitSt();
           ptx::TcFenceBeforeSync();
-          ptx::NamedBarrier(2, kSoftmaxThreads);  // the factors have been read
         }
 #pragma unroll
         for (int c = 0; c < 8; ++c) {  // 128-byte swizzle: chunk c of row r at c ^ (r % 8)
@@ -773,72 +852,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
         if (others > 0 && others < kTile) {
-          if (!BoundedWait(bar(&misc->w_full[0]), g & 1, misc, p.status, 34) || !BoundedWait(bar(&misc->w_full[1]), g & 1, misc, p.status, 34)) ok = false;
+          ok = WarpWait(bar(&misc->w_full), g & 1, misc, p.status, 34) && ok;
           for (int i = row; i < (kTile - others) * kVSlabs * 8; i += kSoftmaxThreads) {
             *reinterpret_cast<int4*>(smem + kOffW + ((i >> 3) & 3) * kSlabBytes + (others + (i >> 5)) * 128 + (i & 7) * 16) = make_int4(0, 0, 0, 0);
           }
         }
-        ptx::FenceProxyAsync();
+        ptx::FenceProxyAsyncShared();
         __syncwarp();
-        if (lane == 0) {
-          ptx::BulkCopyToCta(peer_p_warp, p_warp, 32 * 128, peer_p_bar);
-          ptx::MbarArrive(bar(&misc->p_full));
-        }
+        if (lane == 0) ptx::MbarArrive(bar(&misc->p_full));
+        if (g > 0) ok = WarpWait(bar(&misc->peer_p_empty), (g & 1) ^ 1, misc, p.status, 36) && ok;
+        if (lane == 0) ptx::BulkCopyToCta(peer_p_warp, p_warp, 32 * 128, peer_p_bar);
       }
-      if (gave_up) break;
+      if (!ok) break;
+
+      // The next item's Q first: its first S is then computed under this item's epilogue.
+      more = walk.Next(&next_item, &next_lo, &next_hi);
+      if (more) load_q(next_item);
 
       // ---- epilogue of the item ----
       const float l_all = l_run + exchange(l_run);
-      if (!BoundedWait(bar(&misc->pv_done), (g & 1) ^ 1, misc, p.status, 32)) ok = false;
+      ok = WarpWait(bar(&misc->w_empty), (g & 1) ^ 1, misc, p.status, 32) && ok;
+      if (!ok) break;
       ptx::TcFenceAfterSync();
-      const int n = item.steps();
-      const bool whole = lo == 0 && hi == n;
+      const bool ends = hi == item.steps();
+      const bool whole = lo == 0 && ends;
       const int slot = 2 * run + (lo == 0 ? 1 : 0);
       const int query = which == 0 ? item.q0 : item.q1;
-      misc->factor[row] = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+      const float inv_l = 1.0f / l_all;
+      const bool nothing = l_all == 0.0f;  // no weights, and O may hold anything
       if (rank == 0) {
-        if (row == 0) {
-          if (lo == 0) p.first_run[item.q0] = run;
-          if (hi == n) p.last_run[item.q0] = run;
-        }
+        if (row == 0 && ends && continued) p.merges[run] = make_int4(item.q0, item.q1, misc->began_in, 0);
         if (!whole) {
           p.ws_m[slot * kRows + row] = m_run;
           p.ws_l[slot * kRows + row] = l_all;
         } else if (p.lse != nullptr && query >= 0) {
           p.lse[static_cast<int64_t>(query) * kHeads + head] =
-              l_all == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(m_run) * p.natural + static_cast<double>(logf(l_all)));
+              nothing ? -INFINITY : static_cast<float>(static_cast<double>(m_run) * p.natural + static_cast<double>(logf(l_all)));
         }
       }
-      if (ptx::NamedBarrierOr(1, kSoftmaxThreads, !ok)) {
-        ok = false;
-        break;
-      }
-      const int queries = item.q1 >= 0 ? 2 : 1;
+      continued = false;
+      if (query >= 0) {
 #pragma unroll 1
-      for (int m = 0; m < 2; ++m) {
-        const int dv = kHalf * rank + 128 * m + row;
-#pragma unroll 1
-        for (int c = 0; c < 2 * queries; ++c) {  // 32 rows at a time
+        for (int c = 0; c < kHalf / 32; ++c) {
           uint32_t o[32];
-          ptx::TmemLd32(tmem + lane_base + kColO + 128 * m + 32 * c, o);
+          ptx::TmemLd32(tmem + lane_base + kColO + 32 * c, o);
           ptx::TmemWaitLd();
           if (!whole) {
-            uint4* dst = reinterpret_cast<uint4*>(p.ws_o) + (static_cast<int64_t>(slot) * (kRows / 4) + 8 * c) * kLatent + dv;
+            uint4* dst = reinterpret_cast<uint4*>(p.ws_o) + (static_cast<int64_t>(slot) * (kLatent / 4) + (kHalf * rank + 32 * c) / 4) * kRows + row;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) dst[k * kLatent] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int k = 0; k < 8; ++k) dst[k * kRows] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           } else {
-            __nv_bfloat16* dst = p.out + (static_cast<int64_t>(c < 2 ? item.q0 : item.q1) * kHeads + 32 * (c & 1)) * kLatent + dv;
+            uint4* dst = reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(query) * kHeads + head) * kLatent + kHalf * rank + 32 * c);
+            uint32_t two[16];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float inv = misc->factor[32 * c + k];  // 0: no weights, and the accumulator may hold anything
-              dst[k * kLatent] = __float2bfloat16_rn(inv == 0.0f ? 0.0f : __uint_as_float(o[k]) * inv);
+            for (int k = 0; k < 16; ++k) {
+              const __nv_bfloat162 t = __floats2bfloat162_rn(nothing ? 0.0f : __uint_as_float(o[2 * k]) * inv_l, nothing ? 0.0f : __uint_as_float(o[2 * k + 1]) * inv_l);
+              two[k] = *reinterpret_cast<const uint32_t*>(&t);
             }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) dst[k] = make_uint4(two[4 * k], two[4 * k + 1], two[4 * k + 2], two[4 * k + 3]);
           }
         }
       }
       ptx::TcFenceBeforeSync();
-      ptx::NamedBarrier(2, kSoftmaxThreads);  // the factors have been read
+      __syncwarp();
       if (lane == 0) ptx::MbarArrive(bar(&misc->o_empty));
+    }
+    // The peer's last signals have arrived before this CTA may leave.
+    if (ok && g > 0) {
+      WarpWait(bar(&misc->peer_p_empty), (g & 1) ^ 1, misc, p.status, 37);
+      WarpWait(bar(&misc->p_sent), (g & 1) ^ 1, misc, p.status, 37);
     }
   }
 
@@ -858,116 +941,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 5) ptx::TmemDealloc(tmem, kTmemCols);
 }
 
-// Merges what the runs left of every item that was cut, and writes the result of queries without tokens. A CTA takes one query,
-// four of its heads and 256 / kGroups columns: a thread has one column of the four heads, 16 bytes a part, as the epilogue left
-// them. kGroups groups of threads share the parts out, so that the few queries of a long context have enough loads in flight.
-template <int kGroups>
+// Merges what the runs left of every item that was cut. A CTA takes 32 rows x 32 columns of the item that run blockIdx.y
+// finishes, if another began it; a thread has four columns of a row, 16 bytes a part, a warp's loads 512 contiguous bytes. The
+// result changes places in shared memory so that a row's 64 bytes leave together.
 __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constant__ SharedParams p) {
-  constexpr int kColumns = 256 / kGroups;
-  constexpr int kChunks = kLatent / kColumns;
   constexpr int kBatch = 8;  // parts whose data a thread has in flight
-  const int query = blockIdx.x / (16 * kChunks);
-  const int quad = blockIdx.x / kChunks % 16;
-  const int dv = blockIdx.x % kChunks * kColumns + threadIdx.x % kColumns;
-  const int group = threadIdx.x / kColumns;
-  __shared__ float4 s_acc[kGroups > 1 ? 256 : 1];
+  const int rows = blockIdx.x / (kLatent / 32) * 32, columns = blockIdx.x % (kLatent / 32) * 32;
+  const int lane = threadIdx.x & 31, quad = threadIdx.x >> 5;
+  const int row = rows + lane;
+  __shared__ uint2 s_out[32][9];
   GridDependencyWait();
   GridDependencyTrigger();
-  const bool second = IsSecond(p.leader, query);
-  const int head = second ? query - 1 : query;  // the item's first query
-  __nv_bfloat16* out = p.out + (static_cast<int64_t>(query) * kHeads + 4 * quad) * kLatent + dv;
-  if (ItemAt(p, head).steps() == 0) {
-    if (group == 0) {
+  const int4 merge = p.merges[blockIdx.y];
+  const int query = rows < kHeads ? merge.x : merge.y;
+  if (merge.x < 0 || query < 0) return;
+  const int first = merge.z, last = blockIdx.y;
+  float m = kLowest, l = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const float4* data = p.ws_o + (static_cast<int64_t>(columns) / 4 + quad) * kRows + row;
+  for (int r0 = first; r0 <= last; r0 += kBatch) {
+    float4 d[kBatch];
+    float pm[kBatch], pl[kBatch];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out[i * kLatent] = __float2bfloat16_rn(0.0f);
-      if (dv == 0 && p.lse != nullptr) {
-        for (int i = 0; i < 4; ++i) p.lse[static_cast<int64_t>(query) * kHeads + 4 * quad + i] = -INFINITY;
-      }
-    }
-    return;
-  }
-  const int first = p.first_run[head], last = p.last_run[head];
-  if (first >= last) return;  // one run held it all
-  const int row = (second ? kHeads : 0) + 4 * quad;
-  // Maxima and sums of the parts: part r is run first + r, whose slot is the one it begins in (r = 0) or continues in.
-  float m[4] = {kLowest, kLowest, kLowest, kLowest}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const uint4* ws = reinterpret_cast<const uint4*>(p.ws_o);
-  for (int r0 = first; r0 <= last; r0 += kBatch * kGroups) {
-    uint4 data[kBatch];
-    float4 pm[kBatch], pl[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int r = r0 + k * kGroups + group;
-      const bool there = r <= last && p.has_steps[r] != 0;
+    for (int k = 0; k < kBatch; ++k) {  // part r is run r's, in the slot of the item it begins (the first) or continues
+      const int r = r0 + k;
       const int slot = 2 * r + (r == first ? 1 : 0);
-      pl[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      pm[k] = make_float4(kLowest, kLowest, kLowest, kLowest);
-      data[k] = make_uint4(0, 0, 0, 0);
-      if (there) {
-        pl[k] = *reinterpret_cast<const float4*>(p.ws_l + slot * kRows + row);
-        pm[k] = *reinterpret_cast<const float4*>(p.ws_m + slot * kRows + row);
-        data[k] = ws[(static_cast<int64_t>(slot) * (kRows / 4) + row / 4) * kLatent + dv];
+      pl[k] = 0.0f;
+      if (r <= last) {
+        pl[k] = p.ws_l[slot * kRows + row];
+        pm[k] = p.ws_m[slot * kRows + row];
+        d[k] = data[static_cast<int64_t>(slot) * (kLatent / 4) * kRows];
       }
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const float ml[4] = {pm[k].x, pm[k].y, pm[k].z, pm[k].w}, ll[4] = {pl[k].x, pl[k].y, pl[k].z, pl[k].w};
-      const uint32_t dd[4] = {data[k].x, data[k].y, data[k].z, data[k].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (ll[i] == 0.0f) continue;  // no weights, and the accumulator may hold anything (a NaN sum is not zero)
-        const float big = fmaxf(m[i], ml[i]);
-        const float w_old = exp2f(m[i] - big), w = exp2f(ml[i] - big);
-        acc[i] = acc[i] * w_old + __uint_as_float(dd[i]) * w;
-        l[i] = l[i] * w_old + ll[i] * w;
-        m[i] = big;
-      }
+      if (pl[k] == 0.0f) continue;  // no weights, and the accumulator may hold anything (a NaN sum is not zero)
+      const float big = fmaxf(m, pm[k]);
+      const float w_old = exp2f(m - big), w = exp2f(pm[k] - big);
+      acc.x = acc.x * w_old + d[k].x * w;
+      acc.y = acc.y * w_old + d[k].y * w;
+      acc.z = acc.z * w_old + d[k].z * w;
+      acc.w = acc.w * w_old + d[k].w * w;
+      l = l * w_old + pl[k] * w;
+      m = big;
     }
   }
-  if constexpr (kGroups > 1) {
-    __shared__ float s_m[kGroups][4], s_l[kGroups][4];
-    s_acc[threadIdx.x] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    if (threadIdx.x % kColumns == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s_m[group][i] = m[i];
-        s_l[group][i] = l[i];
-      }
-    }
-    __syncthreads();
-    if (group != 0) return;
-    for (int o = 1; o < kGroups; ++o) {
-      const float4 other = s_acc[o * kColumns + threadIdx.x];
-      const float oa[4] = {other.x, other.y, other.z, other.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float ll = s_l[o][i], ml = s_m[o][i];
-        if (ll == 0.0f) continue;
-        const float big = fmaxf(m[i], ml);
-        const float w_old = exp2f(m[i] - big), w = exp2f(ml - big);
-        acc[i] = acc[i] * w_old + oa[i] * w;
-        l[i] = l[i] * w_old + ll * w;
-        m[i] = big;
-      }
-    }
+  const bool nothing = l == 0.0f;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(nothing ? 0.0f : acc.x / l, nothing ? 0.0f : acc.y / l);
+  const __nv_bfloat162 hi = __floats2bfloat162_rn(nothing ? 0.0f : acc.z / l, nothing ? 0.0f : acc.w / l);
+  s_out[lane][quad] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  if (columns == 0 && quad == 0 && p.lse != nullptr) {
+    p.lse[static_cast<int64_t>(query) * kHeads + (row & (kHeads - 1))] =
+        nothing ? -INFINITY : static_cast<float>(static_cast<double>(m) * p.natural + static_cast<double>(logf(l)));
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i * kLatent] = __float2bfloat16_rn(l[i] == 0.0f ? 0.0f : acc[i] / l[i]);
-  if (dv == 0 && p.lse != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p.lse[static_cast<int64_t>(query) * kHeads + 4 * quad + i] =
-          l[i] == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(m[i]) * p.natural + static_cast<double>(logf(l[i])));
-    }
-  }
+  __syncthreads();
+  const int to = threadIdx.x >> 3, part = threadIdx.x & 7;
+  *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(query) * kHeads + ((rows + to) & (kHeads - 1))) * kLatent + columns + 4 * part) = s_out[to][part];
 }
 
 int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2; }
 
-size_t SharedWorkspaceBytes(int32_t batch) {
+size_t SharedWorkspaceBytes() {
   const size_t slots = static_cast<size_t>(RunsOfDevice()) * 2;
-  return slots * kRows * (kLatent + 2) * sizeof(float) + (2 * static_cast<size_t>(batch) + RunsOfDevice()) * 4 + 64;
+  return slots * kRows * (kLatent + 2) * sizeof(float) + static_cast<size_t>(RunsOfDevice()) * sizeof(int4);
 }
 
 bool SharedSupports(const b200kv_shared_args& a) {
@@ -987,7 +1023,7 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
     configured_device = device;
   }
   CUtensorMap latent_map, rope_map, q_map;
-  if (int32_t rc = GetRowMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, kLatent, kTile, &latent_map)) return rc;
+  if (int32_t rc = GetSlabMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, &latent_map)) return rc;
   if (int32_t rc = GetRowMap(a.pool.rope, a.pool.rope_row_stride, a.pool.pool_rows, kRope, kTile, &rope_map)) return rc;
   if (int32_t rc = GetQMap(a.q, a.q_head_stride, a.q_seq_stride, a.batch, a.heads, kHeads, &q_map)) return rc;
   const int32_t runs = RunsOfDevice();
@@ -1011,22 +1047,18 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.lse = a.lse;
   const size_t slots = static_cast<size_t>(runs) * 2;
-  p.ws_o = static_cast<float*>(a.workspace);
-  p.ws_m = p.ws_o + slots * kRows * kLatent;
+  p.ws_o = static_cast<float4*>(a.workspace);
+  p.ws_m = reinterpret_cast<float*>(p.ws_o + slots * kRows * (kLatent / 4));
   p.ws_l = p.ws_m + slots * kRows;
-  p.first_run = reinterpret_cast<int32_t*>(p.ws_l + slots * kRows);
-  p.last_run = p.first_run + a.batch;
-  p.has_steps = p.last_run + a.batch;
+  p.merges = reinterpret_cast<int4*>(p.ws_l + slots * kRows);
   p.status = status;
   if (int32_t rc = CheckCuda(LaunchOverlapped(MlaDecodeSharedKernel, dim3(2 * static_cast<unsigned>(runs)), dim3(kThreads), kSmemBytes, stream,
                                               latent_map, rope_map, q_map, p),
                              "decode_shared launch")) {
     return rc;
   }
-  const unsigned quads = static_cast<unsigned>(a.batch) * 16;
-  const cudaError_t merged = a.batch <= 4 ? LaunchOverlapped(MlaSharedMergeKernel<4>, dim3(quads * 8), dim3(256), 0, stream, p)
-                                          : LaunchOverlapped(MlaSharedMergeKernel<1>, dim3(quads * 2), dim3(256), 0, stream, p);
-  return CheckCuda(merged, "decode_shared merge launch");
+  return CheckCuda(LaunchOverlapped(MlaSharedMergeKernel, dim3(kRows / 32 * (kLatent / 32), static_cast<unsigned>(runs)), dim3(256), 0, stream, p),
+                   "decode_shared merge launch");
 }
 
 }  // namespace
@@ -1036,7 +1068,7 @@ using namespace b200kv;
 
 extern "C" size_t b200kv_mla_decode_shared_workspace_bytes(int32_t batch, int32_t heads) {
   if (batch <= 0 || heads <= 0) return 0;
-  const size_t own = SharedWorkspaceBytes(batch), plain = b200kv_mla_decode_workspace_bytes(batch, heads, 0);
+  const size_t own = SharedWorkspaceBytes(), plain = b200kv_mla_decode_workspace_bytes(batch, heads, 0);
   return own > plain ? own : plain;
 }
 
@@ -1052,6 +1084,10 @@ extern "C" int32_t b200kv_mla_decode_shared(const b200kv_shared_args* args, void
   if (a.q == nullptr || a.block_table == nullptr || a.kv_len == nullptr || a.leader == nullptr || a.shared_len == nullptr || a.out == nullptr) {
     SetLastError("decode_shared: q, block_table, kv_len, leader, shared_len and out must be non-null");
     return B200KV_ERR_NULLPTR;
+  }
+  if ((reinterpret_cast<uintptr_t>(a.out) & 15u) != 0) {
+    SetLastError("decode_shared refused: out must be 16-byte aligned");
+    return B200KV_ERR_INVALID;
   }
   if (a.batch < 0 || a.heads <= 0 || a.block_size <= 0 || a.max_blocks <= 0 || a.pool.pool_rows % a.block_size != 0 || !(a.scale > 0.0f) ||
       a.q_head_stride < kLatent + kRope || (a.batch > 1 && a.q_seq_stride < 0) || (a.out_fp8 == nullptr) != (a.out_scale == nullptr) ||
@@ -1090,7 +1126,7 @@ extern "C" int32_t b200kv_mla_decode_shared(const b200kv_shared_args* args, void
     d.out_scale = a.out_scale;
     return b200kv_mla_decode(&d, stream, status);
   }
-  const size_t need = SharedWorkspaceBytes(a.batch);
+  const size_t need = SharedWorkspaceBytes();
   if (a.workspace == nullptr || a.workspace_bytes < need || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0) {
     SetLastError("decode_shared: workspace of %zu bytes (16-byte aligned) required, %zu given", need, a.workspace_bytes);
     return a.workspace == nullptr ? B200KV_ERR_NULLPTR : B200KV_ERR_INVALID;

@@ -1480,10 +1480,12 @@ struct MapKeyHash {
 // Row-major [rows][width] bf16 view with row stride `stride` elements; box = 64 columns x box_rows rows (a tile
 // of 64 consecutive rows, or a single row for the loads that gather four rows each), 128-byte swizzle. Maps are
 // cached: a decode step reuses the same 2 x layers views every token.
-int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, CUtensorMap* out) {
+namespace {
+// slabs > 0: the view's columns as that many slabs of 64 along a third axis.
+int32_t CachedRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, int32_t slabs, CUtensorMap* out) {
   static std::mutex mu;
   static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-  const MapKey key{base, stride, rows, width, box_rows};
+  const MapKey key{base, stride, rows, width, slabs > 0 ? -box_rows : box_rows};
   {
     std::lock_guard<std::mutex> lock(mu);
     auto it = cache.find(key);
@@ -1497,12 +1499,12 @@ int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width,
     SetLastError("cuTensorMapEncodeTiled could not be resolved from the CUDA driver");
     return B200KV_ERR_RUNTIME;
   }
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t elem[2] = {1, 1};
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(slabs > 0 ? 64 : width), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(width / 64)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride) * 2, 128};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(slabs)};
+  const cuuint32_t elem[3] = {1, 1, 1};
   CUtensorMap map;
-  const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+  const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, slabs > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box,
                              elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) {
@@ -1517,6 +1519,17 @@ int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width,
   }
   *out = map;
   return B200KV_OK;
+}
+}  // namespace
+
+int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, CUtensorMap* out) {
+  return CachedRowMap(base, stride, rows, width, box_rows, 0, out);
+}
+
+// The latent columns of a pool as eight slabs of 64; box = 64 rows x four slabs, which land one behind the other, each as a box of
+// GetRowMap would.
+int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, CUtensorMap* out) {
+  return CachedRowMap(base, stride, rows, kLatent, kTile, 4, out);
 }
 
 // Query view [batch][heads][576] bf16 with element strides (q_seq_stride, q_head_stride, 1);

@@ -197,6 +197,20 @@ __device__ __forceinline__ void MmaF16SS(uint32_t d_tmem, uint64_t a_desc, uint6
       : "memory");
 }
 
+// The same without touching the accumulator's lanes whose bit is set in off_lo (lanes 0-63, one word for each half of them, both
+// words alike) or off_hi (lanes 64-127).
+__device__ __forceinline__ void MmaF16SSLanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t off_lo, uint32_t off_hi, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %4, %5, %5}, p;\n\t"
+      "}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off_lo), "r"(off_hi), "r"(accumulate)
+      : "memory");
+}
+
 // The same with A in tensor memory: lane = row of A, column = two consecutive elements of its K-major row.
 __device__ __forceinline__ void MmaF16TS(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                          uint32_t accumulate) {
@@ -358,6 +372,13 @@ __device__ __forceinline__ void StClusterV4(uint32_t addr, uint32_t x, uint32_t 
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+__device__ __forceinline__ void LdShared128(uint32_t addr, uint32_t& x, uint32_t& y, uint32_t& z, uint32_t& w) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(w) : "r"(addr) : "memory");
+}
+// Arrival on another CTA's mbarrier (an address in the cluster's shared window).
+__device__ __forceinline__ void MbarArriveRemote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // One 4-byte store into another CTA's shared memory that completes 4 bytes on that CTA's mbarrier.
 __device__ __forceinline__ void StAsyncF32(uint32_t addr, float v, uint32_t bar) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(addr),

@@ -215,7 +215,7 @@ int32_t b200kv_mla_decode(const b200kv_decode_args* args, void* stream, b200kv_s
  * [table_rows][max_blocks], table_rows >= batch without table_index. A bad entry is recorded as B200KV_DEV_BAD_BLOCK (detail =
  * query, column) and reads as zeros. Runs on tensor cores for 64 heads, block_size % 64 == 0 and a 16-byte aligned q with strides
  * that are multiples of 8; any other geometry goes through b200kv_mla_decode (table_index is refused there). q, out, lse, scale,
- * flags, out_fp8 and out_scale as in b200kv_decode_args; workspace of b200kv_mla_decode_shared_workspace_bytes() bytes.
+ * flags, out_fp8 and out_scale as in b200kv_decode_args, out 16-byte aligned; workspace of b200kv_mla_decode_shared_workspace_bytes() bytes.
  */
 typedef struct b200kv_shared_args {
   const void* q;
