@@ -80,7 +80,7 @@ struct Item {
   __device__ __forceinline__ int steps() const { return common + own0 + own1; }
 };
 
-constexpr int kListed = 24;  // items of a run that the cut leaves in shared memory; a run of more walks the arrays again
+constexpr int kListed = 32;  // a run of up to so many items finds them in shared memory
 
 struct Misc {
   uint64_t t_full, t_empty;
@@ -99,15 +99,13 @@ struct Misc {
   uint64_t drain[2];
   uint32_t tmem_base;
   int32_t abort_flag;
-  int32_t start_query;  // the run's first item, its ordinal, the step in it, the run that it began in
-  int32_t start_step;
-  int32_t began_in;
-  int32_t n_items;
-  long long start_ordinal, end_ordinal;
+  int32_t start_step;  // in the run's first item
+  int32_t began_in;    // the run that item began in
+  long long start_ordinal, end_ordinal;  // the run's items
   long long flat_lo, flat_hi;
-  long long scan[8][3];
+  uint2 scan[kThreads / 32];
   float peer_max[2][kRows];
-  Item items[kListed];  // by ordinal % kListed
+  Item items[kListed];  // by ordinal % kListed; a run of more than kListed items reads SharedParams::items
 };
 static_assert(sizeof(Misc) <= kMiscBytes, "Misc does not fit its reservation");
 
@@ -135,17 +133,14 @@ struct SharedParams {
   float4* ws_o;
   float* ws_m;  // [slot][128], log2 domain
   float* ws_l;
+  Item* items;   // [batch]: the items, in order (those of a run are written by the run's CTAs)
   int4* merges;  // [runs]: the item that run c finishes and another began: its queries, the run that began it; x < 0: none
   int32_t* status;
 };
 
 // ---- the list of work -------------------------------------------------------------------------------------------------
-// Query b is the second of a pair if the one before it has the same leader and stands at an even distance from it. What the
+// Query b is the second of a pair if the one before it has the same leader and stands at an even distance from it. Whatever the
 // arrays hold, every query belongs to exactly one item.
-__device__ __forceinline__ bool IsSecond(const int32_t* leader, int b) {
-  return b > 0 && leader[b] == leader[b - 1] && ((static_cast<unsigned>(b - 1) - static_cast<unsigned>(leader[b - 1])) & 1u) == 0;
-}
-
 __device__ __forceinline__ int StepsOf(int tokens) { return tokens > 0 ? (tokens - 1) / kStep + 1 : 0; }
 
 __device__ __forceinline__ Item MakeItem(int q0, int q1, int len0, int len1, int shared0, int shared1) {
@@ -178,9 +173,14 @@ __device__ __forceinline__ Item MakeItem(int q0, int q1, int len0, int len1, int
   return it;
 }
 
-__device__ __forceinline__ Item ItemAt(const SharedParams& p, int b) {  // b: not a second
-  const bool pair = b + 1 < p.batch && IsSecond(p.leader, b + 1);
-  return MakeItem(b, pair ? b + 1 : -1, p.kv_len[b], pair ? p.kv_len[b + 1] : 0, p.shared_len[b], pair ? p.shared_len[b + 1] : 0);
+// The item that begins with query b, without steps if b is the second of a pair. The loads go out together.
+__device__ __forceinline__ Item ItemAt(const SharedParams& p, int b, bool* second) {
+  const int prev = max(b - 1, 0), next = min(b + 1, p.batch - 1);
+  const int lead_prev = p.leader[prev], lead = p.leader[b], lead_next = p.leader[next];
+  const int len0 = p.kv_len[b], len1 = p.kv_len[next], shared0 = p.shared_len[b], shared1 = p.shared_len[next];
+  *second = b > 0 && lead == lead_prev && ((static_cast<unsigned>(prev) - static_cast<unsigned>(lead)) & 1u) == 0;
+  const bool pair = next > b && lead == lead_next && ((static_cast<unsigned>(b) - static_cast<unsigned>(lead)) & 1u) == 0;
+  return MakeItem(b, pair ? next : -1, *second ? 0 : len0, pair && !*second ? len1 : 0, shared0, shared1);
 }
 
 struct Step {
@@ -217,43 +217,38 @@ __device__ __forceinline__ Step StepAt(const Item& it, int s) {
   return st;
 }
 
-// The cut: a step costs 2, entering another item in mid-run 3 more (Q is loaded anew and the accumulators are drained). Step x
-// of the flat list, of the item with ordinal s, stands at cost position 2x + 3s; run c takes the positions
+// The cut: a step costs 2, entering another item in mid-run 6 more (Q is loaded anew and the accumulators are drained). Step x
+// of the flat list, of the item with ordinal s, stands at cost position 2x + 6s; run c takes the positions
 // [ceil(c C / G), ceil((c + 1) C / G)).
 struct Cut {
   long long total_cost;
   long long runs;
-  static constexpr long long kStepCost = 2, kEnterCost = 3;
+  static constexpr long long kStepCost = 2, kEnterCost = 6;
   __device__ static long long Pos(long long x, long long s) { return kStepCost * x + kEnterCost * s; }
-  __device__ long long First(long long c) const { return (c * total_cost + runs - 1) / runs; }
+  // Non-negative quotient; the 32-bit division is several times shorter and covers every realistic size.
+  __device__ static long long Div(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+    return a / b;
+  }
+  __device__ long long First(long long c) const { return Div(c * total_cost + runs - 1, runs); }
+  __device__ long long RunOf(long long pos) const { return Div(pos * runs, total_cost); }
 };
 
 // The items of this run, one after the other. Every role runs the same walk.
 struct Walk {
-  const SharedParams& p;
-  const Misc* misc;
-  int at;         // item of the run, or query where the run has too many to be listed
+  const Item* items;
+  uint32_t at, mask;
   int step;
   long long remaining;
-  bool listed;
-  __device__ Walk(const SharedParams& params, const Misc* m)
-      : p(params), misc(m), step(m->start_step), remaining(m->flat_hi - m->flat_lo), listed(m->n_items <= kListed) {
-    at = listed ? 0 : m->start_query;
+  __device__ Walk(const SharedParams& p, const Misc* misc) : step(misc->start_step), remaining(misc->flat_hi - misc->flat_lo) {
+    const bool listed = misc->end_ordinal - misc->start_ordinal <= kListed;
+    items = listed ? misc->items : p.items;
+    mask = listed ? kListed - 1 : 0xffffffffu;
+    at = static_cast<uint32_t>(misc->start_ordinal);
   }
-  __device__ bool Next(Item* item, int* lo, int* hi) {
+  __device__ __forceinline__ bool Next(Item* item, int* lo, int* hi) {
     if (remaining <= 0) return false;
-    if (listed) {
-      *item = misc->items[(misc->start_ordinal + at) % kListed];
-      ++at;
-    } else {
-      for (;; ++at) {
-        if (at >= p.batch) return false;
-        if (IsSecond(p.leader, at)) continue;
-        *item = ItemAt(p, at);
-        if (item->steps() > 0) break;
-      }
-      ++at;  // (an item that is not finished here is the run's last)
-    }
+    *item = items[at++ & mask];
     *lo = step;
     *hi = static_cast<int>(min(remaining, static_cast<long long>(item->steps() - step))) + step;
     remaining -= *hi - step;
@@ -307,7 +302,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::MbarInit(bar(&misc->peer_p_empty), 1);
     ptx::MbarInit(bar(&misc->o_empty), kSoftmaxWarps);
     misc->abort_flag = 0;
-    misc->start_query = p.batch;
     misc->start_step = 0;
     misc->began_in = 0;
     misc->start_ordinal = misc->end_ordinal = 0;
@@ -326,129 +320,102 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // (let go only after this kernel's own wait: the merge kernel reads the lengths too)
 
   // ---- this run of the list: totals, then the first step at or after the run's first cost position and the next run's ------
-  long long empty = 0;  // items without steps
-  int runs_used;
+  // Two passes of the same scan over the queries, 256 at a time: the first for the totals, the second finds the run's items.
+  bool any_empty = false;
   {
-    long long steps = 0, items = 0;
-    Item mine;
-    int mine_n = 0;  // the first chunk's item of this thread, kept
-    for (int b = threadIdx.x; b < p.batch; b += kThreads) {
-      if (IsSecond(p.leader, b)) continue;
-      const Item it = ItemAt(p, b);
-      const int n = it.steps();
-      if (b < kThreads) {
-        mine = it;
-        mine_n = n;
-      }
-      steps += n;
-      items += n > 0 ? 1 : 0;
-      empty += n > 0 ? 0 : 1;
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      steps += __shfl_xor_sync(0xffffffffu, steps, off);
-      items += __shfl_xor_sync(0xffffffffu, items, off);
-      empty += __shfl_xor_sync(0xffffffffu, empty, off);
-    }
-    if (lane == 0) {
-      misc->scan[warp][0] = steps;
-      misc->scan[warp][1] = items;
-      misc->scan[warp][2] = empty;
-    }
-    __syncthreads();
     long long total = 0, total_items = 0;
-    empty = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      total += misc->scan[w][0];
-      total_items += misc->scan[w][1];
-      empty += misc->scan[w][2];
-    }
-    if (threadIdx.x == 0) {
-      misc->flat_lo = total;
-      misc->flat_hi = total;
-    }
-    const long long cost = Cut::Pos(total, total_items > 0 ? total_items - 1 : 0);
-    // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty.
-    runs_used = static_cast<int>(min(static_cast<long long>(runs), max(1ll, cost / Cut::kStepCost)));
-    const Cut cut{cost, runs_used};
-    const long long k_lo = cut.First(run), k_hi = cut.First(run + 1);
-    long long before = 0, before_items = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-      __syncthreads();
-      const int b = b0 + threadIdx.x;
-      if (b0 > 0) {
-        mine_n = 0;
-        if (b < p.batch && !IsSecond(p.leader, b)) {
-          mine = ItemAt(p, b);
-          mine_n = mine.steps();
-        }
-      }
-      const int n = mine_n;
-      long long incl = n, incl_items = n > 0 ? 1 : 0;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl, off);
-        const long long up_items = __shfl_up_sync(0xffffffffu, incl_items, off);
-        if (lane >= off) {
-          incl += up;
-          incl_items += up_items;
-        }
-      }
-      if (lane == 31) {
-        misc->scan[warp][0] = incl;
-        misc->scan[warp][1] = incl_items;
-      }
-      __syncthreads();
-      long long chunk = 0, chunk_items = 0;
-#pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) {
-          incl += misc->scan[w][0];
-          incl_items += misc->scan[w][1];
-        }
-        chunk += misc->scan[w][0];
-        chunk_items += misc->scan[w][1];
-      }
-      if (n > 0 && run < runs_used) {
-        const long long first = before + incl - n, s = before_items + incl_items - 1;
-        const long long first_pos = Cut::Pos(first, s), last_pos = Cut::Pos(first + n - 1, s);
-        const long long last_before = Cut::Pos(first - 1, s - 1);  // the item before this one ends here
-        auto at_or_after = [&](long long k) {                      // first step at or after cost position k, if it is in this item
-          const long long x = (k - Cut::kEnterCost * s + 1) >> 1;
-          return x > first ? x : first;
-        };
-        if (last_pos >= k_lo && first_pos < k_hi) {
-          misc->items[s % kListed] = mine;  // (more than kListed overwrite each other and are not read)
-          if (s == 0 || last_before < k_lo) {
-            const long long x = at_or_after(k_lo);
-            misc->flat_lo = x;
-            misc->start_query = b;
-            misc->start_step = static_cast<int>(x - first);
-            misc->start_ordinal = s;
-            misc->began_in = static_cast<int>(first_pos * runs_used / cost);
+    Cut cut{};
+    long long k_lo = 0, k_hi = 0;
+    Item mine;
+    int n = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+      long long before = 0, before_items = 0;
+#pragma unroll 1
+      for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+        const int b = b0 + threadIdx.x;
+        if (pass == 0 || p.batch > kThreads) {  // (a batch of one chunk keeps what it has loaded)
+          n = 0;
+          if (b < p.batch) {
+            bool second;
+            mine = ItemAt(p, b, &second);
+            n = mine.steps();
+            any_empty |= n == 0 && !second;
           }
-          atomicMax(reinterpret_cast<unsigned long long*>(&misc->end_ordinal), static_cast<unsigned long long>(s + 1));
         }
-        if (last_pos >= k_hi && (s == 0 || last_before < k_hi)) misc->flat_hi = at_or_after(k_hi);
+        int incl = n, incl_items = n > 0 ? 1 : 0;  // (a query has at most 2^24 + 2 steps, 256 of them fit)
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, incl, off);
+          const int up_items = __shfl_up_sync(0xffffffffu, incl_items, off);
+          if (lane >= off) {
+            incl += up;
+            incl_items += up_items;
+          }
+        }
+        __syncthreads();  // (the chunk before has been read)
+        if (lane == 31) misc->scan[warp] = make_uint2(incl, incl_items);
+        __syncthreads();
+        long long chunk = 0, chunk_items = 0, mine_before = incl - n, mine_items = incl_items - 1;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+          const uint2 of = misc->scan[w];
+          mine_before += w < warp ? of.x : 0;
+          mine_items += w < warp ? of.y : 0;
+          chunk += of.x;
+          chunk_items += of.y;
+        }
+        if (pass == 1 && n > 0) {
+          const long long first = before + mine_before, s = before_items + mine_items;
+          const long long first_pos = Cut::Pos(first, s), last_pos = Cut::Pos(first + n - 1, s);
+          const long long last_before = Cut::Pos(first - 1, s - 1);  // the item before this one ends here
+          auto at_or_after = [&](long long k) {                      // first step at or after cost position k, if it is in this item
+            const long long x = (k - Cut::kEnterCost * s + 1) >> 1;
+            return x > first ? x : first;
+          };
+          if (last_pos >= k_lo && first_pos < k_hi) {
+            misc->items[s % kListed] = mine;  // (of more than kListed the last ones stay, and none is read)
+            if (p.batch > kListed) p.items[s] = mine;
+            if (s == 0 || last_before < k_lo) {
+              const long long x = at_or_after(k_lo);
+              misc->flat_lo = x;
+              misc->start_step = static_cast<int>(x - first);
+              misc->start_ordinal = s;
+              misc->began_in = static_cast<int>(cut.RunOf(first_pos));
+            }
+            atomicMax(reinterpret_cast<unsigned long long*>(&misc->end_ordinal), static_cast<unsigned long long>(s + 1));
+          }
+          if (last_pos >= k_hi && (s == 0 || last_before < k_hi)) misc->flat_hi = at_or_after(k_hi);
+        }
+        before += chunk;
+        before_items += chunk_items;
       }
-      before += chunk;
-      before_items += chunk_items;
+      if (pass == 0) {
+        total = before;
+        total_items = before_items;
+        const long long cost = Cut::Pos(total, total_items > 0 ? total_items - 1 : 0);
+        // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty.
+        cut = Cut{cost, min(static_cast<long long>(runs), max(1ll, cost / Cut::kStepCost))};
+        if (p.batch > kListed) GridDependencyWait();  // (the workspace may be the preceding kernel's too)
+        k_lo = run < cut.runs ? cut.First(run) : cost;
+        k_hi = run < cut.runs ? cut.First(run + 1) : cost;
+        if (threadIdx.x == 0) misc->flat_lo = misc->flat_hi = total;
+      }
     }
   }
-  ptx::TcFenceBeforeSync();
-  __syncthreads();
-  ptx::TcFenceAfterSync();
-  if (threadIdx.x == 0) misc->n_items = static_cast<int>(min(misc->end_ordinal - misc->start_ordinal, 1ll << 30));
   if (p.stable_tables != 0) GridDependencyWait();
   GridDependencyTrigger();
-  __syncthreads();
+  ptx::TcFenceBeforeSync();
+  any_empty = __syncthreads_or(any_empty) != 0;
+  ptx::TcFenceAfterSync();
   ptx::ClusterWait();
   if (threadIdx.x == 0 && rank == 0) p.merges[run] = make_int4(-1, -1, 0, 0);
-  if (empty > 0) {  // queries that attend over nothing, alone or with one like them
+  if (any_empty) {  // queries that attend over nothing, alone or with one like them
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-      const int first = IsSecond(p.leader, b) ? b - 1 : b;
-      if (ItemAt(p, first).steps() > 0) continue;
+      bool second;
+      Item it = ItemAt(p, b, &second);
+      if (second) it = ItemAt(p, b - 1, &second);
+      if (it.steps() > 0) continue;
       int4* out = reinterpret_cast<int4*>(p.out + static_cast<int64_t>(b) * kHeads * kLatent);
       for (int i = threadIdx.x; i < kHeads * kLatent / 8; i += kThreads) out[i] = make_int4(0, 0, 0, 0);
       if (p.lse != nullptr && threadIdx.x < kHeads) p.lse[static_cast<int64_t>(b) * kHeads + threadIdx.x] = -INFINITY;
@@ -767,16 +734,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) ptx::MbarArrive(bar(&misc->qt_full));
     };
-    Item next_item;
-    int next_lo = 0, next_hi = 0;
-    bool more = walk.Next(&next_item, &next_lo, &next_hi);
-    bool continued = misc->start_step > 0;
-    if (more) load_q(next_item);
-    while (ok && more) {
+    bool have = false, continued = misc->start_step > 0;
+    float m_run = kLowest, l_run = 0.0f;
+    for (;;) {
+      // The next item's Q first: its first S is then computed under this item's epilogue.
+      Item next_item;
+      int next_lo, next_hi;
+      const bool more = walk.Next(&next_item, &next_lo, &next_hi);
+      if (more) load_q(next_item);
+      if (have) {
+        // ---- epilogue of the item ----
+        const float l_all = l_run + exchange(l_run);
+        ok = WarpWait(bar(&misc->w_empty), (g & 1) ^ 1, misc, p.status, 32) && ok;
+        weights_free();
+        if (!ok) break;
+        ptx::TcFenceAfterSync();
+        const bool ends = hi == item.steps();
+        const bool whole = lo == 0 && ends;
+        const int slot = 2 * run + (lo == 0 ? 1 : 0);
+        const int query = which == 0 ? item.q0 : item.q1;
+        const float inv_l = 1.0f / l_all;
+        const bool nothing = l_all == 0.0f;  // no weights, and O may hold anything
+        if (rank == 0) {
+          if (row == 0 && ends && continued) p.merges[run] = make_int4(item.q0, item.q1, misc->began_in, 0);
+          if (!whole) {
+            p.ws_m[slot * kRows + row] = m_run;
+            p.ws_l[slot * kRows + row] = l_all;
+          } else if (p.lse != nullptr && query >= 0) {
+            p.lse[static_cast<int64_t>(query) * kHeads + head] =
+                nothing ? -INFINITY : static_cast<float>(static_cast<double>(m_run) * p.natural + static_cast<double>(logf(l_all)));
+          }
+        }
+        continued = false;
+        if (query >= 0) {
+#pragma unroll 1
+          for (int c = 0; c < kHalf / 32; ++c) {
+            uint32_t o[32];
+            ptx::TmemLd32(tmem + lane_base + kColO + 32 * c, o);
+            ptx::TmemWaitLd();
+            if (!whole) {
+              uint4* dst = reinterpret_cast<uint4*>(p.ws_o) + (static_cast<int64_t>(slot) * (kLatent / 4) + (kHalf * rank + 32 * c) / 4) * kRows + row;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) dst[k * kRows] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            } else {
+              // A lane has a row; the rows' 128 bytes (two rounds) change places in the warp's part of the weights' buffer, so that a
+              // store instruction writes four rows' and not a piece of each of 32.
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t two[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const __nv_bfloat162 t = __floats2bfloat162_rn(nothing ? 0.0f : __uint_as_float(o[8 * k + 2 * e]) * inv_l,
+                                                                 nothing ? 0.0f : __uint_as_float(o[8 * k + 2 * e + 1]) * inv_l);
+                  two[e] = *reinterpret_cast<const uint32_t*>(&t);
+                }
+                ptx::StShared128(p_row + (((4 * (c & 1) + k) ^ (row & 7)) << 4), two[0], two[1], two[2], two[3]);
+              }
+              if ((c & 1) != 0) {
+                __syncwarp();
+                const int sub = lane >> 3, chunk = lane & 7;
+                __nv_bfloat16* dst = p.out + (static_cast<int64_t>(query) * kHeads + (warp & 1) * 32 + sub) * kLatent + kHalf * rank + 64 * (c >> 1) + 8 * chunk;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  uint4 v;
+                  ptx::LdShared128(p_warp + (4 * i + sub) * 128 + ((chunk ^ (4 * (i & 1) + sub)) << 4), v.x, v.y, v.z, v.w);
+                  *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(4 * i) * kLatent) = v;
+                }
+                __syncwarp();
+              }
+            }
+          }
+        }
+        ptx::TcFenceBeforeSync();
+        __syncwarp();
+        if (lane == 0) ptx::MbarArrive(bar(&misc->o_empty));
+      }
+      if (!more) break;
       item = next_item;
       lo = next_lo;
       hi = next_hi;
-      float m_run = kLowest, l_run = 0.0f;
+      have = true;
+      m_run = kLowest;
+      l_run = 0.0f;
       for (int s = lo; s < hi && ok; ++s, ++g) {  // (ok is the warp's; warps that give up leave the others' waits to run out)
         const Step st = StepAt(item, s);
         const int mine = max(0, min(kTile, st.valid - kTile * rank)), others = max(0, min(kTile, st.valid - kTile * static_cast<int>(peer)));
@@ -864,59 +903,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) ptx::BulkCopyToCta(peer_p_warp, p_warp, 32 * 128, peer_p_bar);
       }
       if (!ok) break;
-
-      // The next item's Q first: its first S is then computed under this item's epilogue.
-      more = walk.Next(&next_item, &next_lo, &next_hi);
-      if (more) load_q(next_item);
-
-      // ---- epilogue of the item ----
-      const float l_all = l_run + exchange(l_run);
-      ok = WarpWait(bar(&misc->w_empty), (g & 1) ^ 1, misc, p.status, 32) && ok;
-      if (!ok) break;
-      ptx::TcFenceAfterSync();
-      const bool ends = hi == item.steps();
-      const bool whole = lo == 0 && ends;
-      const int slot = 2 * run + (lo == 0 ? 1 : 0);
-      const int query = which == 0 ? item.q0 : item.q1;
-      const float inv_l = 1.0f / l_all;
-      const bool nothing = l_all == 0.0f;  // no weights, and O may hold anything
-      if (rank == 0) {
-        if (row == 0 && ends && continued) p.merges[run] = make_int4(item.q0, item.q1, misc->began_in, 0);
-        if (!whole) {
-          p.ws_m[slot * kRows + row] = m_run;
-          p.ws_l[slot * kRows + row] = l_all;
-        } else if (p.lse != nullptr && query >= 0) {
-          p.lse[static_cast<int64_t>(query) * kHeads + head] =
-              nothing ? -INFINITY : static_cast<float>(static_cast<double>(m_run) * p.natural + static_cast<double>(logf(l_all)));
-        }
-      }
-      continued = false;
-      if (query >= 0) {
-#pragma unroll 1
-        for (int c = 0; c < kHalf / 32; ++c) {
-          uint32_t o[32];
-          ptx::TmemLd32(tmem + lane_base + kColO + 32 * c, o);
-          ptx::TmemWaitLd();
-          if (!whole) {
-            uint4* dst = reinterpret_cast<uint4*>(p.ws_o) + (static_cast<int64_t>(slot) * (kLatent / 4) + (kHalf * rank + 32 * c) / 4) * kRows + row;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) dst[k * kRows] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(query) * kHeads + head) * kLatent + kHalf * rank + 32 * c);
-            uint32_t two[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const __nv_bfloat162 t = __floats2bfloat162_rn(nothing ? 0.0f : __uint_as_float(o[2 * k]) * inv_l, nothing ? 0.0f : __uint_as_float(o[2 * k + 1]) * inv_l);
-              two[k] = *reinterpret_cast<const uint32_t*>(&t);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) dst[k] = make_uint4(two[4 * k], two[4 * k + 1], two[4 * k + 2], two[4 * k + 3]);
-          }
-        }
-      }
-      ptx::TcFenceBeforeSync();
-      __syncwarp();
-      if (lane == 0) ptx::MbarArrive(bar(&misc->o_empty));
     }
     // The peer's last signals have arrived before this CTA may leave.
     if (ok && g > 0) {
@@ -943,52 +929,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // Merges what the runs left of every item that was cut. A CTA takes 32 rows x 32 columns of the item that run blockIdx.y
 // finishes, if another began it; a thread has four columns of a row, 16 bytes a part, a warp's loads 512 contiguous bytes. The
-// result changes places in shared memory so that a row's 64 bytes leave together.
+// first parts' data are on their way while the rows' weights are worked out, once a CTA and not once a thread (twice the time).
+// The result changes places in shared memory so that a row's 64 bytes leave together.
+constexpr int kMergeParts = 128;  // parts whose weights a CTA holds at a time; more than runs there are
 __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constant__ SharedParams p) {
   constexpr int kBatch = 8;  // parts whose data a thread has in flight
   const int rows = blockIdx.x / (kLatent / 32) * 32, columns = blockIdx.x % (kLatent / 32) * 32;
   const int lane = threadIdx.x & 31, quad = threadIdx.x >> 5;
   const int row = rows + lane;
+  __shared__ float s_w[kMergeParts][32];
+  __shared__ float s_m[8][32], s_l[8][32];
   __shared__ uint2 s_out[32][9];
   GridDependencyWait();
   GridDependencyTrigger();
   const int4 merge = p.merges[blockIdx.y];
   const int query = rows < kHeads ? merge.x : merge.y;
   if (merge.x < 0 || query < 0) return;
-  const int first = merge.z, last = blockIdx.y;
-  float m = kLowest, l = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int first = merge.z, parts = static_cast<int>(blockIdx.y) - first + 1;
+  // Part r is run (first + r)'s, in the slot of the item that it begins (the first) or continues.
+  auto slot_of = [&](int r) { return 2 * (first + r) + (r == 0 ? 1 : 0); };
   const float4* data = p.ws_o + (static_cast<int64_t>(columns) / 4 + quad) * kRows + row;
-  for (int r0 = first; r0 <= last; r0 += kBatch) {
-    float4 d[kBatch];
-    float pm[kBatch], pl[kBatch];
+  float4 d[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {  // part r is run r's, in the slot of the item it begins (the first) or continues
-      const int r = r0 + k;
-      const int slot = 2 * r + (r == first ? 1 : 0);
-      pl[k] = 0.0f;
-      if (r <= last) {
-        pl[k] = p.ws_l[slot * kRows + row];
-        pm[k] = p.ws_m[slot * kRows + row];
-        d[k] = data[static_cast<int64_t>(slot) * (kLatent / 4) * kRows];
+  for (int k = 0; k < kBatch; ++k) {
+    if (k < parts) d[k] = data[static_cast<int64_t>(slot_of(k)) * (kLatent / 4) * kRows];
+  }
+  // Warp q takes parts q, q + 8, ..: their sums (kept as weights for now) and the maximum.
+  float m = kLowest;
+  for (int r = quad; r < parts; r += 8) {
+    const float pl = p.ws_l[slot_of(r) * kRows + row], pm = p.ws_m[slot_of(r) * kRows + row];
+    s_w[r][lane] = pm;
+    if (pl != 0.0f) m = fmaxf(m, pm);  // (a part without weights does not count; one whose sum is NaN does)
+  }
+  s_m[quad][lane] = m;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) m = fmaxf(m, s_m[q][lane]);
+  float l = 0.0f;
+  for (int r = quad; r < parts; r += 8) {
+    const float pl = p.ws_l[slot_of(r) * kRows + row];
+    const float w = pl != 0.0f ? exp2f(s_w[r][lane] - m) : 0.0f;
+    s_w[r][lane] = w;
+    l += pl * w;
+  }
+  s_l[quad][lane] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) l += s_l[q][lane];
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int r0 = 0; r0 < parts; r0 += kBatch) {
+    if (r0 > 0) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (r0 + k < parts) d[k] = data[static_cast<int64_t>(slot_of(r0 + k)) * (kLatent / 4) * kRows];
       }
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (pl[k] == 0.0f) continue;  // no weights, and the accumulator may hold anything (a NaN sum is not zero)
-      const float big = fmaxf(m, pm[k]);
-      const float w_old = exp2f(m - big), w = exp2f(pm[k] - big);
-      acc.x = acc.x * w_old + d[k].x * w;
-      acc.y = acc.y * w_old + d[k].y * w;
-      acc.z = acc.z * w_old + d[k].z * w;
-      acc.w = acc.w * w_old + d[k].w * w;
-      l = l * w_old + pl[k] * w;
-      m = big;
+      const float w = r0 + k < parts ? s_w[r0 + k][lane] : 0.0f;
+      if (w == 0.0f) continue;  // no weight, and the accumulator may hold anything
+      acc.x = fmaf(d[k].x, w, acc.x);
+      acc.y = fmaf(d[k].y, w, acc.y);
+      acc.z = fmaf(d[k].z, w, acc.z);
+      acc.w = fmaf(d[k].w, w, acc.w);
     }
   }
   const bool nothing = l == 0.0f;
-  const __nv_bfloat162 lo = __floats2bfloat162_rn(nothing ? 0.0f : acc.x / l, nothing ? 0.0f : acc.y / l);
-  const __nv_bfloat162 hi = __floats2bfloat162_rn(nothing ? 0.0f : acc.z / l, nothing ? 0.0f : acc.w / l);
+  const float inv = 1.0f / l;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(nothing ? 0.0f : acc.x * inv, nothing ? 0.0f : acc.y * inv);
+  const __nv_bfloat162 hi = __floats2bfloat162_rn(nothing ? 0.0f : acc.z * inv, nothing ? 0.0f : acc.w * inv);
   s_out[lane][quad] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
   if (columns == 0 && quad == 0 && p.lse != nullptr) {
     p.lse[static_cast<int64_t>(query) * kHeads + (row & (kHeads - 1))] =
@@ -999,11 +1009,11 @@ __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constan
   *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(query) * kHeads + ((rows + to) & (kHeads - 1))) * kLatent + columns + 4 * part) = s_out[to][part];
 }
 
-int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2; }
+int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2 < kMergeParts ? CurrentDeviceSmCount() / 2 : kMergeParts; }
 
-size_t SharedWorkspaceBytes() {
+size_t SharedWorkspaceBytes(int32_t batch) {
   const size_t slots = static_cast<size_t>(RunsOfDevice()) * 2;
-  return slots * kRows * (kLatent + 2) * sizeof(float) + static_cast<size_t>(RunsOfDevice()) * sizeof(int4);
+  return slots * kRows * (kLatent + 2) * sizeof(float) + static_cast<size_t>(RunsOfDevice()) * sizeof(int4) + static_cast<size_t>(batch) * sizeof(Item);
 }
 
 bool SharedSupports(const b200kv_shared_args& a) {
@@ -1051,6 +1061,7 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   p.ws_m = reinterpret_cast<float*>(p.ws_o + slots * kRows * (kLatent / 4));
   p.ws_l = p.ws_m + slots * kRows;
   p.merges = reinterpret_cast<int4*>(p.ws_l + slots * kRows);
+  p.items = reinterpret_cast<Item*>(p.merges + runs);
   p.status = status;
   if (int32_t rc = CheckCuda(LaunchOverlapped(MlaDecodeSharedKernel, dim3(2 * static_cast<unsigned>(runs)), dim3(kThreads), kSmemBytes, stream,
                                               latent_map, rope_map, q_map, p),
@@ -1068,7 +1079,7 @@ using namespace b200kv;
 
 extern "C" size_t b200kv_mla_decode_shared_workspace_bytes(int32_t batch, int32_t heads) {
   if (batch <= 0 || heads <= 0) return 0;
-  const size_t own = SharedWorkspaceBytes(), plain = b200kv_mla_decode_workspace_bytes(batch, heads, 0);
+  const size_t own = SharedWorkspaceBytes(batch), plain = b200kv_mla_decode_workspace_bytes(batch, heads, 0);
   return own > plain ? own : plain;
 }
 
@@ -1126,7 +1137,7 @@ extern "C" int32_t b200kv_mla_decode_shared(const b200kv_shared_args* args, void
     d.out_scale = a.out_scale;
     return b200kv_mla_decode(&d, stream, status);
   }
-  const size_t need = SharedWorkspaceBytes();
+  const size_t need = SharedWorkspaceBytes(a.batch);
   if (a.workspace == nullptr || a.workspace_bytes < need || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0) {
     SetLastError("decode_shared: workspace of %zu bytes (16-byte aligned) required, %zu given", need, a.workspace_bytes);
     return a.workspace == nullptr ? B200KV_ERR_NULLPTR : B200KV_ERR_INVALID;
