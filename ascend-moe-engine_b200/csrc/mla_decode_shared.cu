@@ -134,7 +134,10 @@ struct SharedParams {
   float* ws_m;  // [slot][128], log2 domain
   float* ws_l;
   Item* items;   // [batch]: the items, in order (those of a run are written by the run's CTAs)
-  int4* merges;  // [runs]: the item that run c finishes and another began: its queries, the run that began it; x < 0: none
+  // What there is to merge: an item's queries, the run that began it, the run that finished it; x < 0: nothing. By the item's
+  // first query where the batch has no more queries than there are runs, else by the run that finished it.
+  int4* merges;
+  int32_t merges_by_query;
   int32_t* status;
 };
 
@@ -409,13 +412,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   any_empty = __syncthreads_or(any_empty) != 0;
   ptx::TcFenceAfterSync();
   ptx::ClusterWait();
-  if (threadIdx.x == 0 && rank == 0) p.merges[run] = make_int4(-1, -1, 0, 0);
+  if (threadIdx.x == 0 && rank == 0 && p.merges_by_query == 0) p.merges[run] = make_int4(-1, -1, 0, 0);
   if (any_empty) {  // queries that attend over nothing, alone or with one like them
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
       bool second;
       Item it = ItemAt(p, b, &second);
       if (second) it = ItemAt(p, b - 1, &second);
       if (it.steps() > 0) continue;
+      if (threadIdx.x == 0 && p.merges_by_query != 0) p.merges[b] = make_int4(-1, -1, 0, 0);
       int4* out = reinterpret_cast<int4*>(p.out + static_cast<int64_t>(b) * kHeads * kLatent);
       for (int i = threadIdx.x; i < kHeads * kLatent / 8; i += kThreads) out[i] = make_int4(0, 0, 0, 0);
       if (p.lse != nullptr && threadIdx.x < kHeads) p.lse[static_cast<int64_t>(b) * kHeads + threadIdx.x] = -INFINITY;
@@ -756,7 +760,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const float inv_l = 1.0f / l_all;
         const bool nothing = l_all == 0.0f;  // no weights, and O may hold anything
         if (rank == 0) {
-          if (row == 0 && ends && continued) p.merges[run] = make_int4(item.q0, item.q1, misc->began_in, 0);
+          if (row == 0 && ends) {
+            if (p.merges_by_query != 0) {
+              p.merges[item.q0] = continued ? make_int4(item.q0, item.q1, misc->began_in, run) : make_int4(-1, -1, 0, 0);
+              if (item.q1 >= 0) p.merges[item.q1] = make_int4(-1, -1, 0, 0);
+            } else if (continued) {
+              p.merges[run] = make_int4(item.q0, item.q1, misc->began_in, run);
+            }
+          }
           if (!whole) {
             p.ws_m[slot * kRows + row] = m_run;
             p.ws_l[slot * kRows + row] = l_all;
@@ -927,86 +938,122 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 5) ptx::TmemDealloc(tmem, kTmemCols);
 }
 
-// Merges what the runs left of every item that was cut. A CTA takes 32 rows x 32 columns of the item that run blockIdx.y
-// finishes, if another began it; a thread has four columns of a row, 16 bytes a part, a warp's loads 512 contiguous bytes. The
-// first parts' data are on their way while the rows' weights are worked out, once a CTA and not once a thread (twice the time).
-// The result changes places in shared memory so that a row's 64 bytes leave together.
-constexpr int kMergeParts = 128;  // parts whose weights a CTA holds at a time; more than runs there are
+// Merges what the runs left of every item that was cut. A CTA takes 32 rows x kColumns columns of one. A warp has eight rows x four
+// quads of columns: it reads 128 bytes of a quad's rows and writes 32 bytes of a row, and goes over the strips of 16 columns of its
+// half of the CTA's columns. The rows' weights are worked out once, by the whole CTA.
+constexpr int kMergeParts = 128;  // more than runs there are
+constexpr int kMergeRows = 32;
+
+// kStrips strips of kParts parts are in flight at a time: eight loads a thread, whatever the number of parts.
+template <int kAllStrips, int kStrips, int kParts>
+__device__ __forceinline__ void MergeStrips(const float4* data, const int64_t (&strip)[2], int first, int parts, const float* weight, float inv,
+                                            __nv_bfloat16* out) {
+#pragma unroll 1
+  for (int s0 = 0; s0 < kAllStrips; s0 += kStrips) {
+    float4 acc[kStrips];
+#pragma unroll
+    for (int s = 0; s < kStrips; ++s) acc[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int r0 = 0; r0 < parts; r0 += kParts) {
+      float4 d[kStrips][kParts];
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) {
+#pragma unroll
+        for (int s = 0; s < kStrips; ++s) {
+          // Part r is run (first + r)'s, in the slot of the item that it begins (the first) or continues.
+          if (r0 + k < parts) d[s][k] = data[(2 * (first + r0 + k) + (r0 + k == 0 ? 1 : 0)) * strip[0] + (s0 + s) * strip[1]];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) {
+        const float w = r0 + k < parts ? weight[(r0 + k) * kMergeRows] : 0.0f;
+        if (w == 0.0f) continue;  // no weight, and the accumulator may hold anything
+#pragma unroll
+        for (int s = 0; s < kStrips; ++s) {
+          acc[s].x = fmaf(d[s][k].x, w, acc[s].x);
+          acc[s].y = fmaf(d[s][k].y, w, acc[s].y);
+          acc[s].z = fmaf(d[s][k].z, w, acc[s].z);
+          acc[s].w = fmaf(d[s][k].w, w, acc[s].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kStrips; ++s) {
+      const bool nothing = inv == 0.0f;  // a row without weights
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(nothing ? 0.0f : acc[s].x * inv, nothing ? 0.0f : acc[s].y * inv);
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(nothing ? 0.0f : acc[s].z * inv, nothing ? 0.0f : acc[s].w * inv);
+      *reinterpret_cast<uint2*>(out + 16 * (s0 + s)) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  }
+}
+
+template <int kColumns>
 __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constant__ SharedParams p) {
-  constexpr int kBatch = 8;  // parts whose data a thread has in flight
-  const int rows = blockIdx.x / (kLatent / 32) * 32, columns = blockIdx.x % (kLatent / 32) * 32;
-  const int lane = threadIdx.x & 31, quad = threadIdx.x >> 5;
-  const int row = rows + lane;
-  __shared__ float s_w[kMergeParts][32];
-  __shared__ float s_m[8][32], s_l[8][32];
-  __shared__ uint2 s_out[32][9];
+  const int rows = blockIdx.x / (kLatent / kColumns) * kMergeRows, columns = blockIdx.x % (kLatent / kColumns) * kColumns;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float s_w[kMergeParts][kMergeRows];
+  __shared__ float s_m[8][kMergeRows], s_l[8][kMergeRows];
   GridDependencyWait();
   GridDependencyTrigger();
   const int4 merge = p.merges[blockIdx.y];
   const int query = rows < kHeads ? merge.x : merge.y;
   if (merge.x < 0 || query < 0) return;
-  const int first = merge.z, parts = static_cast<int>(blockIdx.y) - first + 1;
-  // Part r is run (first + r)'s, in the slot of the item that it begins (the first) or continues.
-  auto slot_of = [&](int r) { return 2 * (first + r) + (r == 0 ? 1 : 0); };
-  const float4* data = p.ws_o + (static_cast<int64_t>(columns) / 4 + quad) * kRows + row;
-  float4 d[kBatch];
+  const int first = merge.z, parts = merge.w - first + 1;
+  float l;
+  {
+    // Warp w takes parts w, w + 8, ..; a lane has a row.
+    const int row = rows + lane;
+    float m = kLowest, pl[kMergeParts / 8];
 #pragma unroll
-  for (int k = 0; k < kBatch; ++k) {
-    if (k < parts) d[k] = data[static_cast<int64_t>(slot_of(k)) * (kLatent / 4) * kRows];
-  }
-  // Warp q takes parts q, q + 8, ..: their sums (kept as weights for now) and the maximum.
-  float m = kLowest;
-  for (int r = quad; r < parts; r += 8) {
-    const float pl = p.ws_l[slot_of(r) * kRows + row], pm = p.ws_m[slot_of(r) * kRows + row];
-    s_w[r][lane] = pm;
-    if (pl != 0.0f) m = fmaxf(m, pm);  // (a part without weights does not count; one whose sum is NaN does)
-  }
-  s_m[quad][lane] = m;
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < 8; ++q) m = fmaxf(m, s_m[q][lane]);
-  float l = 0.0f;
-  for (int r = quad; r < parts; r += 8) {
-    const float pl = p.ws_l[slot_of(r) * kRows + row];
-    const float w = pl != 0.0f ? exp2f(s_w[r][lane] - m) : 0.0f;
-    s_w[r][lane] = w;
-    l += pl * w;
-  }
-  s_l[quad][lane] = l;
-  __syncthreads();
-  l = 0.0f;
-#pragma unroll
-  for (int q = 0; q < 8; ++q) l += s_l[q][lane];
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int r0 = 0; r0 < parts; r0 += kBatch) {
-    if (r0 > 0) {
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (r0 + k < parts) d[k] = data[static_cast<int64_t>(slot_of(r0 + k)) * (kLatent / 4) * kRows];
-      }
+    for (int i = 0; i < kMergeParts / 8; ++i) {
+      const int r = 8 * i + warp;
+      pl[i] = 0.0f;
+      if (r >= parts) break;
+      const int at = (2 * (first + r) + (r == 0 ? 1 : 0)) * kRows + row;
+      pl[i] = p.ws_l[at];
+      const float pm = p.ws_m[at];
+      s_w[r][lane] = pm;
+      if (pl[i] != 0.0f) m = fmaxf(m, pm);  // (a part without weights does not count; one whose sum is NaN does)
     }
+    s_m[warp][lane] = m;
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const float w = r0 + k < parts ? s_w[r0 + k][lane] : 0.0f;
-      if (w == 0.0f) continue;  // no weight, and the accumulator may hold anything
-      acc.x = fmaf(d[k].x, w, acc.x);
-      acc.y = fmaf(d[k].y, w, acc.y);
-      acc.z = fmaf(d[k].z, w, acc.z);
-      acc.w = fmaf(d[k].w, w, acc.w);
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, s_m[w][lane]);
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMergeParts / 8; ++i) {
+      const int r = 8 * i + warp;
+      if (r >= parts) break;
+      const float w = pl[i] != 0.0f ? exp2f(s_w[r][lane] - m) : 0.0f;
+      s_w[r][lane] = w;
+      l += pl[i] * w;
+    }
+    s_l[warp][lane] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) l += s_l[w][lane];
+    if (columns == 0 && warp == 0 && p.lse != nullptr) {
+      p.lse[static_cast<int64_t>(query) * kHeads + (row & (kHeads - 1))] =
+          l == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(m) * p.natural + static_cast<double>(logf(l)));
     }
   }
-  const bool nothing = l == 0.0f;
-  const float inv = 1.0f / l;
-  const __nv_bfloat162 lo = __floats2bfloat162_rn(nothing ? 0.0f : acc.x * inv, nothing ? 0.0f : acc.y * inv);
-  const __nv_bfloat162 hi = __floats2bfloat162_rn(nothing ? 0.0f : acc.z * inv, nothing ? 0.0f : acc.w * inv);
-  s_out[lane][quad] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-  if (columns == 0 && quad == 0 && p.lse != nullptr) {
-    p.lse[static_cast<int64_t>(query) * kHeads + (row & (kHeads - 1))] =
-        nothing ? -INFINITY : static_cast<float>(static_cast<double>(m) * p.natural + static_cast<double>(logf(l)));
+  const int mine = 8 * (warp & 3) + (lane & 7);                                      // this thread's row of the 32
+  const int quad = columns / 4 + (warp >> 2) * (kColumns / 8) + (lane >> 3);    // and its first quad of columns
+  l = __shfl_sync(0xffffffffu, l, mine);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float4* data = p.ws_o + static_cast<int64_t>(quad) * kRows + rows + mine;
+  const int64_t strip[2] = {static_cast<int64_t>(kLatent / 4) * kRows, 4 * kRows};  // from slot to slot, from strip to strip
+  __nv_bfloat16* out = p.out + (static_cast<int64_t>(query) * kHeads + ((rows + mine) & (kHeads - 1))) * kLatent + 4 * quad;
+  const float* weight = &s_w[0][mine];
+  constexpr int kStrips = kColumns / 32;
+  if (kStrips >= 4 && parts <= 2) {
+    MergeStrips<kStrips, kStrips >= 4 ? 4 : 1, 2>(data, strip, first, parts, weight, inv, out);
+  } else if (kStrips >= 2 && parts <= 4) {
+    MergeStrips<kStrips, kStrips >= 2 ? 2 : 1, 4>(data, strip, first, parts, weight, inv, out);
+  } else {
+    MergeStrips<kStrips, 1, 8>(data, strip, first, parts, weight, inv, out);
   }
-  __syncthreads();
-  const int to = threadIdx.x >> 3, part = threadIdx.x & 7;
-  *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(query) * kHeads + ((rows + to) & (kHeads - 1))) * kLatent + columns + 4 * part) = s_out[to][part];
 }
 
 int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2 < kMergeParts ? CurrentDeviceSmCount() / 2 : kMergeParts; }
@@ -1062,13 +1109,23 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   p.ws_l = p.ws_m + slots * kRows;
   p.merges = reinterpret_cast<int4*>(p.ws_l + slots * kRows);
   p.items = reinterpret_cast<Item*>(p.merges + runs);
+  p.merges_by_query = a.batch <= runs ? 1 : 0;
   p.status = status;
   if (int32_t rc = CheckCuda(LaunchOverlapped(MlaDecodeSharedKernel, dim3(2 * static_cast<unsigned>(runs)), dim3(kThreads), kSmemBytes, stream,
                                               latent_map, rope_map, q_map, p),
                              "decode_shared launch")) {
     return rc;
   }
-  return CheckCuda(LaunchOverlapped(MlaSharedMergeKernel, dim3(kRows / 32 * (kLatent / 32), static_cast<unsigned>(runs)), dim3(256), 0, stream, p),
+  // The fewer queries, the fewer items there can be to merge, and the more parts they have: fewer columns a CTA, so that half the
+  // queries' items give some four CTAs an SM.
+  const unsigned merges = static_cast<unsigned>(a.batch < runs ? a.batch : runs);
+  auto merge = [&](auto kernel, int columns) {
+    return LaunchOverlapped(kernel, dim3(static_cast<unsigned>(kRows / kMergeRows * (kLatent / columns)), merges), dim3(256), 0, stream, p);
+  };
+  return CheckCuda(a.batch < 37   ? merge(MlaSharedMergeKernel<32>, 32)
+                   : a.batch < 74 ? merge(MlaSharedMergeKernel<64>, 64)
+                   : a.batch < 148 ? merge(MlaSharedMergeKernel<128>, 128)
+                                   : merge(MlaSharedMergeKernel<256>, 256),
                    "decode_shared merge launch");
 }
 
