@@ -193,6 +193,19 @@ def _load() -> ctypes.CDLL:
         fn.argtypes = [c_void_p, c_int32]
     lib.b200kv_block_pool_grow.restype = c_int32
     lib.b200kv_block_pool_grow.argtypes = [c_void_p, c_int32, c_int32, c_void_p]
+    lib.b200kv_block_pool_ungrow.restype = c_int32
+    lib.b200kv_block_pool_ungrow.argtypes = [c_void_p, c_int32, c_int32]
+    lib.b200kv_block_pool_fork.restype = c_int32
+    lib.b200kv_block_pool_fork.argtypes = [c_void_p, c_int32, c_int32, c_int32, c_void_p]
+    lib.b200kv_block_pool_unshare.restype = c_int32
+    lib.b200kv_block_pool_unshare.argtypes = [c_void_p, c_int32, c_int32, c_void_p]
+    for name in ("plan_compact", "apply_moves"):
+        fn = getattr(lib, f"b200kv_block_pool_{name}")
+        fn.restype = c_int32
+    lib.b200kv_block_pool_plan_compact.argtypes = [c_void_p, c_int32, c_void_p]
+    lib.b200kv_block_pool_apply_moves.argtypes = [c_void_p, c_void_p, c_int32]
+    lib.b200kv_block_pool_ref_count.restype = c_int32
+    lib.b200kv_block_pool_ref_count.argtypes = [c_void_p, c_int32]
     lib.b200kv_block_pool_free_count.restype = c_int32
     lib.b200kv_block_pool_free_count.argtypes = [c_void_p]
     lib.b200kv_block_pool_seq_len.restype = c_int32
@@ -529,6 +542,45 @@ class BlockPool:
     def release(self, seq: int) -> None:
         check(lib.b200kv_block_pool_release(self._h, seq))
 
+    def ungrow(self, seq: int, n_tokens: int) -> None:
+        check(lib.b200kv_block_pool_ungrow(self._h, seq, n_tokens))
+
+    def _move(self, call, *args):
+        import numpy as np
+
+        move = np.empty((1, 3), dtype=np.int32)
+        check(call(self._h, *args, move.ctypes.data))
+        return move if move[0, 0] >= 0 else move[:0]
+
+    def fork(self, src: int, dst: int, n_tokens: int = -1):
+        """dst begins as the first n_tokens of src (-1: all) and shares its whole blocks. Returns the moves that are still to be
+        made on the device, int32 [0 or 1, 3] for copy_blocks: the half-filled block's."""
+        return self._move(lib.b200kv_block_pool_fork, src, dst, n_tokens)
+
+    def unshare(self, seq: int, index: int):
+        """A block of its own for seq in place of its block `index`; returns the moves still to be made, as fork does."""
+        return self._move(lib.b200kv_block_pool_unshare, seq, index)
+
+    def plan_compact(self, max_moves: int = -1):
+        """Moves int32 [n, 3] of used blocks towards the pool's start; apply_moves changes the tables once they are enqueued."""
+        import numpy as np
+
+        most = self.num_blocks if max_moves < 0 else max_moves
+        moves = np.empty((max(most, 1), 3), dtype=np.int32)
+        n = int(lib.b200kv_block_pool_plan_compact(self._h, most, moves.ctypes.data))
+        if n < 0:
+            raise B200KVError(-n, last_error())
+        return moves[:n].copy()
+
+    def apply_moves(self, moves) -> None:
+        import numpy as np
+
+        moves = np.ascontiguousarray(moves, dtype=np.int32).reshape(-1, 3)
+        check(lib.b200kv_block_pool_apply_moves(self._h, moves.ctypes.data, len(moves)))
+
+    def ref_count(self, block: int) -> int:
+        return int(lib.b200kv_block_pool_ref_count(self._h, block))
+
     def validate(self) -> None:
         check(lib.b200kv_block_pool_validate(self._h))
 
@@ -742,6 +794,13 @@ class Engine:
         lib.b200kv_engine_layer_attend.restype = c_int32
         lib.b200kv_engine_layer_attend.argtypes = [c_void_p, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                                                    c_void_p, c_void_p]
+        lib.b200kv_engine_fork.restype = c_int32
+        lib.b200kv_engine_fork.argtypes = [c_void_p, c_int32, c_int32, c_int32, c_void_p]
+        for name in ("trim", "compact"):
+            fn = getattr(lib, f"b200kv_engine_{name}")
+            fn.restype = c_int32
+        lib.b200kv_engine_trim.argtypes = [c_void_p, c_int32, c_int32, c_void_p]
+        lib.b200kv_engine_compact.argtypes = [c_void_p, c_int32, c_void_p]
         lib.b200kv_engine_end_step.restype = c_int32
         lib.b200kv_engine_end_step.argtypes = [c_void_p]
         lib.b200kv_engine_stats_json.restype = c_int64
@@ -820,6 +879,24 @@ class Engine:
 
     def end_step(self):
         check(lib.b200kv_engine_end_step(self._h))
+
+    def _stream(self, stream):
+        return _stream_handle(stream) if self.config.backend == 0 else None
+
+    def fork(self, src: int, dst: int, n_tokens: int = -1, stream=None):
+        """dst begins as the first n_tokens of src (-1: all), sharing its whole blocks; the half-filled one is copied."""
+        check(lib.b200kv_engine_fork(self._h, src, dst, n_tokens, self._stream(stream)))
+
+    def trim(self, seq: int, n_tokens: int, stream=None):
+        """Takes back the last n_tokens of seq (rejected drafts)."""
+        check(lib.b200kv_engine_trim(self._h, seq, n_tokens, self._stream(stream)))
+
+    def compact(self, max_moves: int = -1, stream=None) -> int:
+        """Moves up to max_moves blocks (-1: all that stand behind a free one) towards the pool's start; returns how many."""
+        n = int(lib.b200kv_engine_compact(self._h, max_moves, self._stream(stream)))
+        if n < 0:
+            raise B200KVError(-n, last_error())
+        return n
 
     def abort_step(self):
         lib.b200kv_engine_abort_step.restype = c_int32

@@ -36,7 +36,8 @@ struct b200kv_block_pool {
   int32_t* lens;         // tokens per sequence
   int32_t* used_blocks;  // table entries in use per sequence
   uint8_t* live;
-  uint8_t* scratch;      // [num_blocks] ownership marks for Validate
+  int32_t* refs;         // [num_blocks] table entries that name the block: more than one once a sequence has been forked
+  int32_t* scratch;      // [num_blocks] for Validate and for compacting
 };
 
 extern "C" b200kv_block_pool* b200kv_block_pool_create(int32_t num_blocks, int32_t block_size, int32_t max_seqs,
@@ -60,8 +61,9 @@ extern "C" b200kv_block_pool* b200kv_block_pool_create(int32_t num_blocks, int32
   pool->lens = new (std::nothrow) int32_t[max_seqs]();
   pool->used_blocks = new (std::nothrow) int32_t[max_seqs]();
   pool->live = new (std::nothrow) uint8_t[max_seqs]();
-  pool->scratch = new (std::nothrow) uint8_t[num_blocks]();
-  if (!pool->ring || !pool->table || !pool->lens || !pool->used_blocks || !pool->live || !pool->scratch) {
+  pool->refs = new (std::nothrow) int32_t[num_blocks]();
+  pool->scratch = new (std::nothrow) int32_t[num_blocks]();
+  if (!pool->ring || !pool->table || !pool->lens || !pool->used_blocks || !pool->live || !pool->refs || !pool->scratch) {
     SetLastError("block pool: host allocation failed");
     b200kv_block_pool_destroy(pool);
     return nullptr;
@@ -76,7 +78,6 @@ extern "C" b200kv_block_pool* b200kv_block_pool_create(int32_t num_blocks, int32
     pool->scratch[id] = 1;
     pool->ring[i] = id;
   }
-  std::memset(pool->scratch, 0, static_cast<size_t>(num_blocks));
   pool->head = 0;
   pool->free_count = num_blocks;
   return pool;
@@ -89,6 +90,7 @@ extern "C" void b200kv_block_pool_destroy(b200kv_block_pool* pool) {
   delete[] pool->lens;
   delete[] pool->used_blocks;
   delete[] pool->live;
+  delete[] pool->refs;
   delete[] pool->scratch;
   delete pool;
 }
@@ -104,6 +106,38 @@ bool SeqInRange(const b200kv_block_pool* pool, int32_t seq, const char* what) {
     return false;
   }
   return true;
+}
+
+int32_t TakeFree(b200kv_block_pool* pool) {
+  const int32_t id = pool->ring[pool->head];
+  pool->head = pool->head + 1 == pool->num_blocks ? 0 : pool->head + 1;
+  --pool->free_count;
+  pool->refs[id] = 1;
+  return id;
+}
+
+// One table entry less for a block; the last one gives it back, to the front of the free list or to its end.
+void Drop(b200kv_block_pool* pool, int32_t id, bool to_front) {
+  if (--pool->refs[id] > 0) return;
+  if (to_front) {
+    pool->head = pool->head == 0 ? pool->num_blocks - 1 : pool->head - 1;
+    pool->ring[pool->head] = id;
+  } else {
+    int32_t tail = pool->head + pool->free_count;
+    if (tail >= pool->num_blocks) tail -= pool->num_blocks;
+    pool->ring[tail] = id;
+  }
+  ++pool->free_count;
+}
+
+int32_t RowsIn(const b200kv_block_pool* pool, int32_t seq, int32_t index) {  // tokens of the sequence in its block `index`
+  const int64_t left = pool->lens[seq] - static_cast<int64_t>(index) * pool->block_size;
+  return static_cast<int32_t>(left < pool->block_size ? left : pool->block_size);
+}
+
+void NoMove(int32_t* move) {
+  move[0] = move[1] = -1;
+  move[2] = 0;
 }
 }  // namespace
 
@@ -141,13 +175,13 @@ extern "C" int32_t b200kv_block_pool_grow(b200kv_block_pool* pool, int32_t seq, 
                  pool->free_count, pool->num_blocks);
     return B200KV_ERR_INVALID;
   }
-  // Commit.
   int32_t* row = pool->table + static_cast<size_t>(seq) * pool->max_blocks_per_seq;
-  for (int64_t i = have; i < need; ++i) {
-    row[i] = pool->ring[pool->head];
-    pool->head = pool->head + 1 == pool->num_blocks ? 0 : pool->head + 1;
-    --pool->free_count;
+  if (n_tokens > 0 && pool->lens[seq] % pool->block_size != 0 && pool->refs[row[have - 1]] > 1) {
+    SetLastError("grow: the last block of sequence %d (%d, half filled) belongs to others too: unshare it first", seq, row[have - 1]);
+    return B200KV_ERR_INVALID;
   }
+  // Commit.
+  for (int64_t i = have; i < need; ++i) row[i] = TakeFree(pool);
   pool->used_blocks[seq] = static_cast<int32_t>(need);
   const int32_t old_len = pool->lens[seq];
   for (int32_t k = 0; k < n_tokens; ++k) {
@@ -158,8 +192,8 @@ extern "C" int32_t b200kv_block_pool_grow(b200kv_block_pool* pool, int32_t seq, 
   return B200KV_OK;
 }
 
-// Takes back the last n_tokens of a sequence and returns the blocks that empties to the FRONT of the free
-// list, newest first: undoing the most recent grows in reverse order restores tables, lengths and the free
+// Takes back the last n_tokens of a sequence and returns the blocks that empties (and no other sequence holds) to the FRONT of the
+// free list, newest first: undoing the most recent grows in reverse order restores tables, lengths and the free
 // list exactly (a step that is abandoned half way leaves no trace).
 extern "C" int32_t b200kv_block_pool_ungrow(b200kv_block_pool* pool, int32_t seq, int32_t n_tokens) {
   if (!SeqInRange(pool, seq, "ungrow")) return pool ? B200KV_ERR_INVALID : B200KV_ERR_NULLPTR;
@@ -172,9 +206,7 @@ extern "C" int32_t b200kv_block_pool_ungrow(b200kv_block_pool* pool, int32_t seq
   const int32_t keep = (new_len + pool->block_size - 1) / pool->block_size;
   int32_t* row = pool->table + static_cast<size_t>(seq) * pool->max_blocks_per_seq;
   for (int32_t i = pool->used_blocks[seq] - 1; i >= keep; --i) {
-    pool->head = pool->head == 0 ? pool->num_blocks - 1 : pool->head - 1;
-    pool->ring[pool->head] = row[i];
-    ++pool->free_count;
+    Drop(pool, row[i], true);
     row[i] = 0;
   }
   pool->used_blocks[seq] = keep;
@@ -189,18 +221,171 @@ extern "C" int32_t b200kv_block_pool_release(b200kv_block_pool* pool, int32_t se
     return B200KV_ERR_INVALID;
   }
   int32_t* row = pool->table + static_cast<size_t>(seq) * pool->max_blocks_per_seq;
-  int32_t tail = pool->head + pool->free_count;
-  if (tail >= pool->num_blocks) tail -= pool->num_blocks;
   for (int32_t i = 0; i < pool->used_blocks[seq]; ++i) {
-    pool->ring[tail] = row[i];
-    tail = tail + 1 == pool->num_blocks ? 0 : tail + 1;
-    ++pool->free_count;
+    Drop(pool, row[i], false);
     row[i] = 0;
   }
   pool->used_blocks[seq] = 0;
   pool->lens[seq] = 0;
   pool->live[seq] = 0;
   return B200KV_OK;
+}
+
+// A sequence that begins as the first n_tokens of another: whole blocks are held by both, the half-filled one behind them is a block
+// of its own, whose rows are the caller's to copy.
+extern "C" int32_t b200kv_block_pool_fork(b200kv_block_pool* pool, int32_t src, int32_t dst, int32_t n_tokens, int32_t* move_out) {
+  if (!SeqInRange(pool, src, "fork") || !SeqInRange(pool, dst, "fork")) return pool ? B200KV_ERR_INVALID : B200KV_ERR_NULLPTR;
+  if (move_out == nullptr) {
+    SetLastError("fork: move_out is null");
+    return B200KV_ERR_NULLPTR;
+  }
+  if (!pool->live[src] || pool->live[dst] || n_tokens < -1 || n_tokens > pool->lens[src]) {
+    SetLastError("fork: sequence %d live=%d with %d tokens, %d asked for, into sequence %d live=%d", src, static_cast<int>(pool->live[src]),
+                 pool->lens[src], n_tokens, dst, static_cast<int>(pool->live[dst]));
+    return B200KV_ERR_INVALID;
+  }
+  const int32_t n = n_tokens < 0 ? pool->lens[src] : n_tokens;
+  const int32_t whole = n / pool->block_size, rest = n % pool->block_size;
+  if (rest > 0 && pool->free_count == 0) {
+    SetLastError("fork: %d tokens end inside a block, and none of %d is free for the copy", n, pool->num_blocks);
+    return B200KV_ERR_INVALID;
+  }
+  const int32_t* from = pool->table + static_cast<size_t>(src) * pool->max_blocks_per_seq;
+  int32_t* to = pool->table + static_cast<size_t>(dst) * pool->max_blocks_per_seq;
+  for (int32_t i = 0; i < whole; ++i) {
+    to[i] = from[i];
+    ++pool->refs[from[i]];
+  }
+  NoMove(move_out);
+  if (rest > 0) {
+    to[whole] = TakeFree(pool);
+    move_out[0] = from[whole];
+    move_out[1] = to[whole];
+    move_out[2] = rest;
+  }
+  pool->live[dst] = 1;
+  pool->lens[dst] = n;
+  pool->used_blocks[dst] = whole + (rest > 0 ? 1 : 0);
+  return B200KV_OK;
+}
+
+// Gives a sequence a block of its own in place of its block `index`, if others hold that one too; its rows are the caller's to copy.
+extern "C" int32_t b200kv_block_pool_unshare(b200kv_block_pool* pool, int32_t seq, int32_t index, int32_t* move_out) {
+  if (!SeqInRange(pool, seq, "unshare")) return pool ? B200KV_ERR_INVALID : B200KV_ERR_NULLPTR;
+  if (move_out == nullptr) {
+    SetLastError("unshare: move_out is null");
+    return B200KV_ERR_NULLPTR;
+  }
+  if (!pool->live[seq] || index < 0 || index >= pool->used_blocks[seq]) {
+    SetLastError("unshare: sequence %d live=%d has %d blocks, not one with index %d", seq, static_cast<int>(pool->live[seq]), pool->used_blocks[seq],
+                 index);
+    return B200KV_ERR_INVALID;
+  }
+  NoMove(move_out);
+  int32_t* entry = pool->table + static_cast<size_t>(seq) * pool->max_blocks_per_seq + index;
+  if (pool->refs[*entry] == 1) return B200KV_OK;
+  if (pool->free_count == 0) {
+    SetLastError("unshare: no block of %d is free for the copy of block %d", pool->num_blocks, *entry);
+    return B200KV_ERR_INVALID;
+  }
+  move_out[0] = *entry;
+  move_out[2] = RowsIn(pool, seq, index);
+  --pool->refs[*entry];
+  *entry = TakeFree(pool);
+  move_out[1] = *entry;
+  return B200KV_OK;
+}
+
+// Undoes the unshare that has just been made, when its copy could not be (not part of the C ABI).
+namespace b200kv {
+void UndoUnshare(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move) {
+  if (move[0] < 0) return;
+  Drop(pool, move[1], true);
+  pool->table[static_cast<size_t>(seq) * pool->max_blocks_per_seq + index] = move[0];
+  ++pool->refs[move[0]];
+}
+}  // namespace b200kv
+
+// The used blocks with the highest ids, each with the lowest free id below it: done to the end, the used blocks are 0 .. used - 1.
+extern "C" int32_t b200kv_block_pool_plan_compact(b200kv_block_pool* pool, int32_t max_moves, int32_t* moves_out) {
+  if (pool == nullptr) {
+    SetLastError("plan_compact: pool is null");
+    return -B200KV_ERR_NULLPTR;
+  }
+  if (max_moves < 0 || (max_moves > 0 && moves_out == nullptr)) {
+    SetLastError("plan_compact: %d moves into %p", max_moves, static_cast<void*>(moves_out));
+    return moves_out == nullptr ? -B200KV_ERR_NULLPTR : -B200KV_ERR_INVALID;
+  }
+  // The rows that mean something: what the sequence with the most tokens in a block has there.
+  std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
+  for (int32_t s = 0; s < pool->max_seqs; ++s) {
+    const int32_t* row = pool->table + static_cast<size_t>(s) * pool->max_blocks_per_seq;
+    for (int32_t i = 0; i < pool->used_blocks[s]; ++i) {
+      const int32_t rows = RowsIn(pool, s, i);
+      if (rows > pool->scratch[row[i]]) pool->scratch[row[i]] = rows;
+    }
+  }
+  int32_t n = 0, to = 0;
+  for (int32_t from = pool->num_blocks - 1; n < max_moves; --from) {
+    while (from > to && pool->refs[from] == 0) --from;
+    while (to < from && pool->refs[to] > 0) ++to;
+    if (to >= from) break;
+    moves_out[3 * n] = from;
+    moves_out[3 * n + 1] = to++;
+    moves_out[3 * n + 2] = pool->scratch[from];
+    ++n;
+  }
+  return n;
+}
+
+// The tables after the moves: every entry of a source names its destination, the sources are free. The free list is in the order of
+// the ids afterwards.
+extern "C" int32_t b200kv_block_pool_apply_moves(b200kv_block_pool* pool, const int32_t* moves, int32_t n_moves) {
+  if (pool == nullptr || (n_moves > 0 && moves == nullptr)) {
+    SetLastError("apply_moves: pool and moves must be non-null");
+    return B200KV_ERR_NULLPTR;
+  }
+  // Plan: sources in use, destinations free, none twice. scratch[id]: 0 untouched, destination + 1 of a source, -1 a destination.
+  std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
+  for (int32_t i = 0; i < n_moves; ++i) {
+    const int32_t from = moves[3 * i], to = moves[3 * i + 1];
+    if (from < 0 || from >= pool->num_blocks || to < 0 || to >= pool->num_blocks || pool->refs[from] == 0 || pool->refs[to] != 0 ||
+        pool->scratch[from] != 0 || pool->scratch[to] != 0) {
+      SetLastError("apply_moves: move %d from block %d to block %d (a block in use to a free one, no block twice)", i, from, to);
+      return B200KV_ERR_INVALID;
+    }
+    pool->scratch[from] = to + 1;
+    pool->scratch[to] = -1;
+  }
+  if (n_moves < 0) {
+    SetLastError("apply_moves: %d moves", n_moves);
+    return B200KV_ERR_INVALID;
+  }
+  if (n_moves == 0) return B200KV_OK;
+  for (int32_t s = 0; s < pool->max_seqs; ++s) {
+    int32_t* row = pool->table + static_cast<size_t>(s) * pool->max_blocks_per_seq;
+    for (int32_t i = 0; i < pool->used_blocks[s]; ++i) {
+      if (pool->scratch[row[i]] > 0) row[i] = pool->scratch[row[i]] - 1;
+    }
+  }
+  for (int32_t i = 0; i < n_moves; ++i) {
+    pool->refs[moves[3 * i + 1]] = pool->refs[moves[3 * i]];
+    pool->refs[moves[3 * i]] = 0;
+  }
+  pool->head = 0;
+  int32_t n = 0;
+  for (int32_t id = 0; id < pool->num_blocks; ++id) {
+    if (pool->refs[id] == 0) pool->ring[n++] = id;
+  }
+  return B200KV_OK;
+}
+
+extern "C" int32_t b200kv_block_pool_ref_count(const b200kv_block_pool* pool, int32_t block) {
+  if (pool == nullptr || block < 0 || block >= pool->num_blocks) {
+    SetLastError("ref_count: block %d outside the pool", block);
+    return -1;
+  }
+  return pool->refs[block];
 }
 
 extern "C" int32_t b200kv_block_pool_free_count(const b200kv_block_pool* pool) {
@@ -234,16 +419,16 @@ extern "C" int32_t b200kv_block_pool_validate(const b200kv_block_pool* pool) {
     SetLastError("validate: pool is null");
     return B200KV_ERR_NULLPTR;
   }
-  std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks));
+  std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
   int64_t owned = 0;
   int32_t at = pool->head;
   for (int32_t i = 0; i < pool->free_count; ++i) {
     const int32_t id = pool->ring[at];
-    if (id < 0 || id >= pool->num_blocks || pool->scratch[id]) {
-      SetLastError("validate: free-list entry %d holds block %d (out of range or listed twice)", i, id);
+    if (id < 0 || id >= pool->num_blocks || pool->scratch[id] || pool->refs[id] != 0) {
+      SetLastError("validate: free-list entry %d holds block %d (out of range, listed twice or in use)", i, id);
       return B200KV_ERR_INVALID;
     }
-    pool->scratch[id] = 1;
+    pool->scratch[id] = -1;
     at = at + 1 == pool->num_blocks ? 0 : at + 1;
   }
   for (int32_t s = 0; s < pool->max_seqs; ++s) {
@@ -263,12 +448,18 @@ extern "C" int32_t b200kv_block_pool_validate(const b200kv_block_pool* pool) {
     }
     for (int32_t i = 0; i < pool->used_blocks[s]; ++i) {
       const int32_t id = row[i];
-      if (id < 0 || id >= pool->num_blocks || pool->scratch[id]) {
-        SetLastError("validate: sequence %d entry %d holds block %d (out of range or owned twice)", s, i, id);
+      if (id < 0 || id >= pool->num_blocks || pool->scratch[id] < 0) {
+        SetLastError("validate: sequence %d entry %d holds block %d (out of range or free)", s, i, id);
         return B200KV_ERR_INVALID;
       }
-      pool->scratch[id] = 1;
-      ++owned;
+      if (pool->scratch[id]++ == 0) ++owned;
+    }
+  }
+  for (int32_t id = 0; id < pool->num_blocks; ++id) {
+    const int32_t named = pool->scratch[id] < 0 ? 0 : pool->scratch[id];
+    if (named != pool->refs[id]) {
+      SetLastError("validate: block %d is named by %d table entries, %d are counted", id, named, pool->refs[id]);
+      return B200KV_ERR_INVALID;
     }
   }
   if (owned + pool->free_count != pool->num_blocks) {

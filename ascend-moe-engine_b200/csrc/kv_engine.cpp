@@ -12,8 +12,11 @@
 //              order: producer (kv_a_norm + rope + kv_cache_write, stages 6-8), attention (9), MX quantisation of
 //              its output (10). end: no allocation happened since begin, as the reference asserts per step
 //              (:502-503, 535-536).
+//   between steps  fork: a sequence that begins as another's first tokens and shares its whole blocks; trim: rejected
+//              drafts are taken back; compact: blocks move towards the pool's start. What has to be copied on the device is
+//              enqueued before the tables change for good.
 // Every device operation is one of the library's own entry points (b200kv_append_fused, b200kv_mla_decode,
-// b200kv_mx_quant_e4m3); this file is host logic only and allocates nothing after Build.
+// b200kv_mla_decode_shared, b200kv_copy_blocks); this file is host logic only and allocates nothing after Build.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -27,6 +30,7 @@ namespace b200kv {
 void SetLastError(const char* fmt, ...);
 int32_t CheckCuda(cudaError_t err, const char* what);
 int32_t FaultCheck(const char* entry_point);
+void UndoUnshare(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move);
 }  // namespace b200kv
 
 using b200kv::CheckCuda;
@@ -38,12 +42,17 @@ struct b200kv_engine {
   b200kv_kv_cache cache{};
   b200kv_block_pool* pool = nullptr;
   int64_t status_handle = -1;
+  int64_t queries_handle = -1;
+  int64_t moves_handle = -1;
   // Device addresses of the step's spans (resolved once, after Commit).
   int32_t* d_table = nullptr;
   int32_t* d_slots = nullptr;
   int32_t* d_lens = nullptr;
   int32_t* d_status = nullptr;
-  // One pinned block that mirrors [table .. lens] of the arena byte for byte: one copy uploads a step.
+  int32_t* d_queries = nullptr;  // [4][max_step_tokens]: kv_len, leader, shared_len, table_index of the step's queries
+  int32_t* d_moves = nullptr;    // [num_blocks][3]
+  // One pinned block that mirrors [queries | table .. lens] of the arena byte for byte: one copy uploads a step (from the
+  // table on, when the step's attention needs no queries).
   unsigned char* staging = nullptr;
   size_t staging_bytes = 0;
   size_t table_off = 0, slots_off = 0, lens_off = 0;
@@ -56,13 +65,96 @@ struct b200kv_engine {
   int64_t active_tokens = 0;
   std::vector<int32_t> step_seq_ids;   // sized at Build: the step's sequences and by how much each grew
   std::vector<int32_t> step_grown;
+  bool step_shares = false;            // the step's attention is b200kv_mla_decode_shared
+  std::vector<int32_t> moves;          // [num_blocks][3], sized at Build
 };
 
 namespace {
 
+// Common tokens of neighbours from which attention goes through the entry point for shared rows (a quarter of all tokens as well).
+constexpr int64_t kLeastCommon = 16384;
+
 int32_t Refuse(const char* text) {
   SetLastError("%s", text);
   return B200KV_ERR_INVALID;
+}
+
+// The queries of the step in the staging block: one per new token, attending over its sequence up to itself. A sequence's tokens
+// are a group; so are neighbours of one token each whose table rows begin with the same blocks. True when attention should go
+// through the entry point for shared rows: always with several tokens a sequence, else when the common blocks are worth it.
+bool PlanQueries(b200kv_engine* e, int32_t n_seqs, int32_t n_tokens) {
+  const size_t stride = static_cast<size_t>(e->cfg.max_step_tokens);
+  int32_t* kv_len = reinterpret_cast<int32_t*>(e->staging);
+  int32_t *leader = kv_len + stride, *shared = leader + stride, *index = shared + stride;
+  const int32_t* table = reinterpret_cast<const int32_t*>(e->staging + e->table_off);
+  const int32_t* lens = reinterpret_cast<const int32_t*>(e->staging + e->lens_off);
+  const int64_t columns = e->cfg.max_blocks_per_seq;
+  if (n_tokens != n_seqs) {
+    int32_t at = 0;
+    for (int32_t i = 0; i < n_seqs; ++i) {
+      const int32_t n = e->step_grown[static_cast<size_t>(i)], first = at;
+      for (int32_t k = 0; k < n; ++k, ++at) {
+        kv_len[at] = lens[i] - n + k + 1;
+        leader[at] = first;
+        shared[at] = lens[i];
+        index[at] = i;
+      }
+    }
+    return true;
+  }
+  int64_t all = 0, common = 0;  // tokens: of all queries, and those that a pair reads once instead of twice
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    kv_len[i] = lens[i];
+    index[i] = i;
+    leader[i] = i;
+    shared[i] = 0;
+    all += lens[i];
+  }
+  for (int32_t i = 0; i + 1 < n_seqs;) {
+    // Pair by pair, as the kernel takes them: the two rows' common blocks, of which the new tokens' own are none.
+    const int32_t *a = table + i * columns, *b = table + (i + 1) * columns;
+    const int64_t most = (lens[i] < lens[i + 1] ? lens[i] : lens[i + 1]) / e->cfg.block_size;
+    int64_t blocks = 0;
+    while (blocks < most && a[blocks] == b[blocks]) ++blocks;
+    if (blocks == 0) {
+      ++i;
+      continue;
+    }
+    leader[i + 1] = i;
+    shared[i] = shared[i + 1] = static_cast<int32_t>(blocks * e->cfg.block_size);
+    common += shared[i];
+    i += 2;
+  }
+  return common >= kLeastCommon && 4 * common >= all;
+}
+
+// Moves of blocks (pool ids) in every layer, enqueued on the stream.
+int32_t CopyMoves(b200kv_engine* e, const int32_t* moves, int32_t n, void* stream) {
+  if (n == 0) return B200KV_OK;
+  b200kv_pool_view view;
+  if (int32_t rc = b200kv_kv_cache_layer_view(e->arena, &e->cache, 0, &view)) return rc;
+  const size_t bytes = static_cast<size_t>(n) * 12;
+  const int64_t rows = static_cast<int64_t>(e->cfg.num_blocks) * e->cfg.block_size;
+  if (e->cfg.backend != B200KV_ARENA_DEVICE) {  // host memory stands for the device's
+    if (int32_t rc = b200kv::FaultCheck("b200kv_copy_blocks")) return rc;
+    for (int64_t l = 0; l < e->cfg.layers; ++l) {
+      for (int32_t i = 0; i < n; ++i) {
+        const int64_t from = moves[3 * i] * static_cast<int64_t>(e->cfg.block_size), to = moves[3 * i + 1] * static_cast<int64_t>(e->cfg.block_size);
+        auto copy = [&](void* base, int64_t width) {
+          auto* layer = static_cast<unsigned char*>(base) + l * rows * width;
+          std::memcpy(layer + to * width, layer + from * width, static_cast<size_t>(moves[3 * i + 2] * width));
+        };
+        copy(view.latent, B200KV_LATENT_DIM * 2);
+        copy(view.rope, B200KV_ROPE_DIM * 2);
+      }
+    }
+    return B200KV_OK;
+  }
+  // (from pageable memory: the list has been read when the call returns, so that the next one may be written)
+  if (int32_t rc = CheckCuda(cudaMemcpyAsync(e->d_moves, moves, bytes, cudaMemcpyHostToDevice, static_cast<cudaStream_t>(stream)), "engine moves upload"))
+    return rc;
+  return b200kv_copy_blocks(&view, e->cfg.layers, rows * B200KV_LATENT_DIM, rows * B200KV_ROPE_DIM, e->d_moves, n, e->cfg.block_size, stream,
+                            e->d_status);
 }
 
 }  // namespace
@@ -91,17 +183,26 @@ extern "C" b200kv_engine* b200kv_engine_create(const b200kv_engine_config* confi
   };
   e->arena = b200kv_arena_create(c.backend);
   if (e->arena == nullptr) return fail();
-  // RESERVE: the KV spans (table, slots, lengths, the two layer-major caches), then the status word.
+  // RESERVE: the step's queries, the KV spans (table, slots, lengths, the two layer-major caches), then the status word and
+  // the moves of a compaction.
+  e->queries_handle = b200kv_arena_reserve(e->arena, "kv.queries", static_cast<size_t>(c.max_step_tokens) * 16, 0);
+  if (e->queries_handle < 0) return fail();
   if (b200kv_kv_cache_reserve_batched(e->arena, c.num_blocks, c.block_size, c.layers, c.max_seqs, c.max_blocks_per_seq,
                                       c.max_step_tokens, &e->cache) != B200KV_OK) {
     return fail();
   }
   e->status_handle = b200kv_arena_reserve(e->arena, "kv.status", 16, 0);
   if (e->status_handle < 0) return fail();
+  e->moves_handle = b200kv_arena_reserve(e->arena, "kv.moves", static_cast<size_t>(c.num_blocks) * 12, 0);
+  if (e->moves_handle < 0) return fail();
   // The attention workspace is the only operator workspace of this path (the producer and the quantiser need
-  // none): its high-water mark, one commit, the workspace, the latch.
-  const size_t workspace = c.backend == B200KV_ARENA_DEVICE ? b200kv_mla_decode_workspace_bytes(c.max_seqs, B200KV_HEADS, 0)
-                                                            : 4096;
+  // none): its high-water mark over both attention entry points, one commit, the workspace, the latch.
+  size_t workspace = 4096;
+  if (c.backend == B200KV_ARENA_DEVICE) {
+    workspace = b200kv_mla_decode_shared_workspace_bytes(c.max_step_tokens, B200KV_HEADS);
+    const size_t plain = b200kv_mla_decode_workspace_bytes(c.max_seqs, B200KV_HEADS, 0);
+    if (plain > workspace) workspace = plain;
+  }
   if (b200kv_arena_note_workspace(e->arena, workspace) != B200KV_OK || b200kv_arena_commit(e->arena) != B200KV_OK ||
       b200kv_arena_commit_workspace(e->arena) != B200KV_OK) {
     return fail();
@@ -110,11 +211,12 @@ extern "C" b200kv_engine* b200kv_engine_create(const b200kv_engine_config* confi
   e->d_slots = static_cast<int32_t*>(b200kv_arena_address(e->arena, e->cache.slot_mapping_handle));
   e->d_lens = static_cast<int32_t*>(b200kv_arena_address(e->arena, e->cache.seq_lens_handle));
   e->d_status = static_cast<int32_t*>(b200kv_arena_address(e->arena, e->status_handle));
-  e->table_off = 0;
-  e->slots_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.slot_mapping_handle) -
-                                     b200kv_arena_offset(e->arena, e->cache.block_table_handle));
-  e->lens_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.seq_lens_handle) -
-                                    b200kv_arena_offset(e->arena, e->cache.block_table_handle));
+  e->d_queries = static_cast<int32_t*>(b200kv_arena_address(e->arena, e->queries_handle));
+  e->d_moves = static_cast<int32_t*>(b200kv_arena_address(e->arena, e->moves_handle));
+  const int64_t first = b200kv_arena_offset(e->arena, e->queries_handle);
+  e->table_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.block_table_handle) - first);
+  e->slots_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.slot_mapping_handle) - first);
+  e->lens_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.seq_lens_handle) - first);
   e->staging_bytes = e->lens_off + static_cast<size_t>(c.max_seqs) * 4;
   if (c.backend == B200KV_ARENA_DEVICE) {
     void* pinned = nullptr;
@@ -129,6 +231,7 @@ extern "C" b200kv_engine* b200kv_engine_create(const b200kv_engine_config* confi
   if (e->pool == nullptr) return fail();
   e->step_seq_ids.resize(static_cast<size_t>(c.max_seqs));
   e->step_grown.resize(static_cast<size_t>(c.max_seqs));
+  e->moves.resize(static_cast<size_t>(c.num_blocks) * 3);
   if (b200kv_arena_seal(e->arena) != B200KV_OK) return fail();
   return e;
 }
@@ -223,19 +326,22 @@ extern "C" int32_t b200kv_engine_begin_step(b200kv_engine* e, const int32_t* seq
     e->step_grown[static_cast<size_t>(i)] = n;
   }
   for (int32_t i = at; i < e->cfg.max_step_tokens; ++i) s_slots[i] = -1;  // padding rows write nothing
+  e->step_shares = PlanQueries(e, n_seqs, at);
   e->allocations_at_begin = b200kv_arena_allocations(e->arena);
   e->step_seqs = n_seqs;
   e->step_tokens = at;
-  // ONE upload per step: the table rows, the slots and the lengths lie in the arena in this order. An upload
+  // ONE upload per step: the queries, the table rows, the slots and the lengths lie in the arena in this order. An upload
   // that fails takes the step's growth back: the call changed nothing.
+  const size_t from = e->step_shares ? 0 : e->table_off;
+  unsigned char* to = reinterpret_cast<unsigned char*>(e->d_queries) + from;
   int32_t rc = b200kv::FaultCheck("b200kv_engine_step_upload");
   if (rc == B200KV_OK) {
     if (e->cfg.backend == B200KV_ARENA_DEVICE) {
-      rc = CheckCuda(cudaMemcpyAsync(e->d_table, e->staging, e->staging_bytes, cudaMemcpyHostToDevice,
+      rc = CheckCuda(cudaMemcpyAsync(to, e->staging + from, e->staging_bytes - from, cudaMemcpyHostToDevice,
                                      static_cast<cudaStream_t>(stream)),
                      "engine step upload");
     } else {
-      std::memcpy(e->d_table, e->staging, e->staging_bytes);
+      std::memcpy(to, e->staging + from, e->staging_bytes - from);
     }
   }
   if (rc != B200KV_OK) {
@@ -292,8 +398,33 @@ extern "C" int32_t b200kv_engine_layer_attend(b200kv_engine* e, int32_t layer, c
                                               void* stream) {
   if (e == nullptr) return B200KV_ERR_NULLPTR;
   if (!e->in_step) return Refuse("engine_layer_attend: no step in flight");
-  if (e->step_tokens != e->step_seqs) {
-    return Refuse("engine_layer_attend: decode attention takes one new token per sequence (this step is a prefill chunk)");
+  if (out_fp8 != nullptr && out_scales == nullptr) return Refuse("engine_layer_attend: out_fp8 without out_scales");
+  if (e->step_shares) {
+    b200kv_shared_args a{};
+    if (int32_t rc = b200kv_kv_cache_layer_view(e->arena, &e->cache, layer, &a.pool)) return rc;
+    const int64_t stride = e->cfg.max_step_tokens;
+    a.q = q;
+    a.q_seq_stride = q_seq_stride;
+    a.q_head_stride = q_head_stride;
+    a.block_table = e->d_table;
+    a.max_blocks = e->cfg.max_blocks_per_seq;
+    a.table_rows = e->cfg.max_seqs;
+    a.kv_len = e->d_queries;
+    a.leader = e->d_queries + stride;
+    a.shared_len = e->d_queries + 2 * stride;
+    a.table_index = e->d_queries + 3 * stride;
+    a.batch = e->step_tokens;
+    a.heads = B200KV_HEADS;
+    a.block_size = e->cfg.block_size;
+    a.scale = e->cfg.scale;
+    a.out = out;
+    a.workspace = b200kv_arena_workspace(e->arena);
+    a.workspace_bytes = static_cast<size_t>(b200kv_arena_workspace_bytes(e->arena));
+    a.flags = B200KV_DECODE_STABLE_TABLES;
+    a.out_fp8 = out_fp8;
+    a.out_scale = out_fp8 != nullptr ? out_scales : nullptr;
+    if (int32_t rc = b200kv_arena_workspace_fits(e->arena, b200kv_mla_decode_shared_workspace_bytes(a.batch, a.heads))) return rc;
+    return b200kv_mla_decode_shared(&a, stream, e->d_status);
   }
   b200kv_decode_args a{};
   if (int32_t rc = b200kv_kv_cache_layer_view(e->arena, &e->cache, layer, &a.pool)) return rc;
@@ -318,9 +449,61 @@ extern "C" int32_t b200kv_engine_layer_attend(b200kv_engine* e, int32_t layer, c
   // the attention call: the kernel that writes `out` quantises what it writes.
   a.out_fp8 = out_fp8;
   a.out_scale = out_fp8 != nullptr ? out_scales : nullptr;
-  if (out_fp8 != nullptr && out_scales == nullptr) return Refuse("engine_layer_attend: out_fp8 without out_scales");
   if (int32_t rc = b200kv_arena_workspace_fits(e->arena, b200kv_mla_decode_workspace_bytes(a.batch, a.heads, 0))) return rc;
   return b200kv_mla_decode(&a, stream, e->d_status);
+}
+
+extern "C" int32_t b200kv_engine_fork(b200kv_engine* e, int32_t src, int32_t dst, int32_t n_tokens, void* stream) {
+  if (e == nullptr) return B200KV_ERR_NULLPTR;
+  if (e->in_step) return Refuse("engine_fork: a step is in flight");
+  int32_t move[3];
+  if (int32_t rc = b200kv_block_pool_fork(e->pool, src, dst, n_tokens, move)) return rc;
+  if (move[0] >= 0) {
+    if (int32_t rc = CopyMoves(e, move, 1, stream)) {
+      b200kv_block_pool_ungrow(e->pool, dst, move[2]);  // (its own block first, to the front of the free list)
+      b200kv_block_pool_release(e->pool, dst);
+      return rc;
+    }
+  }
+  e->active_tokens += b200kv_block_pool_seq_len(e->pool, dst);
+  return B200KV_OK;
+}
+
+extern "C" int32_t b200kv_engine_trim(b200kv_engine* e, int32_t seq, int32_t n_tokens, void* stream) {
+  if (e == nullptr) return B200KV_ERR_NULLPTR;
+  if (e->in_step) return Refuse("engine_trim: a step is in flight");
+  const int32_t len = b200kv_block_pool_seq_len(e->pool, seq);
+  if (len < 0 || n_tokens < 0 || n_tokens > len) {
+    SetLastError("engine_trim: sequence %d holds %d tokens (-1: not admitted), %d to take back", seq, len, n_tokens);
+    return B200KV_ERR_INVALID;
+  }
+  const int32_t left = len - n_tokens;
+  if (n_tokens > 0 && left % e->cfg.block_size != 0) {  // the block that will be half filled is the sequence's own from here on
+    const int32_t index = left / e->cfg.block_size;
+    int32_t move[3];
+    if (int32_t rc = b200kv_block_pool_unshare(e->pool, seq, index, move)) return rc;
+    if (move[0] >= 0) {
+      if (move[2] > left % e->cfg.block_size) move[2] = left % e->cfg.block_size;
+      if (int32_t rc = CopyMoves(e, move, 1, stream)) {
+        b200kv::UndoUnshare(e->pool, seq, index, move);
+        return rc;
+      }
+    }
+  }
+  if (int32_t rc = b200kv_block_pool_ungrow(e->pool, seq, n_tokens)) return rc;
+  e->active_tokens -= n_tokens;
+  return B200KV_OK;
+}
+
+extern "C" int32_t b200kv_engine_compact(b200kv_engine* e, int32_t max_moves, void* stream) {
+  if (e == nullptr) return -B200KV_ERR_NULLPTR;
+  if (e->in_step) return -Refuse("engine_compact: a step is in flight");
+  const int32_t most = max_moves < 0 || max_moves > e->cfg.num_blocks ? e->cfg.num_blocks : max_moves;
+  const int32_t n = b200kv_block_pool_plan_compact(e->pool, most, e->moves.data());
+  if (n <= 0) return n;
+  if (int32_t rc = CopyMoves(e, e->moves.data(), n, stream)) return -rc;
+  if (int32_t rc = b200kv_block_pool_apply_moves(e->pool, e->moves.data(), n)) return -rc;  // cannot fail after the plan
+  return n;
 }
 
 extern "C" int32_t b200kv_engine_end_step(b200kv_engine* e) {

@@ -468,6 +468,23 @@ int32_t b200kv_block_pool_release(b200kv_block_pool* pool, int32_t seq);
 /* Takes back the last n_tokens of `seq`; blocks that empties return to the FRONT of the free list, so that undoing
  * the most recent grows in reverse order restores tables, lengths and the free list exactly. */
 int32_t b200kv_block_pool_ungrow(b200kv_block_pool* pool, int32_t seq, int32_t n_tokens);
+/*
+ * Sequences that share blocks. A move is {source block, destination block, rows}: what the caller still has to copy on the device
+ * (b200kv_copy_blocks, in every layer), {-1, -1, 0} for nothing. A block is free again when the last sequence that holds it lets go
+ * of it (release, ungrow).
+ *   fork          `dst` (not admitted) begins as the first n_tokens of `src` (-1: all): whole blocks are held by both, a
+ *                 half-filled one is copied into a block of `dst`'s own.
+ *   unshare       `seq` gets a block of its own in place of its block `index`, if others hold that one too. grow refuses to write
+ *                 into a half-filled block that others hold (what an ungrow into a common block leaves).
+ *   plan_compact  up to max_moves moves of the used blocks with the highest ids to the lowest free ids, [max_moves][3]; returns how
+ *                 many (or a negated error code) and changes nothing. apply_moves changes the tables accordingly, once the copies
+ *                 are enqueued; the free list is in the order of the ids afterwards.
+ */
+int32_t b200kv_block_pool_fork(b200kv_block_pool* pool, int32_t src, int32_t dst, int32_t n_tokens, int32_t* move_out);
+int32_t b200kv_block_pool_unshare(b200kv_block_pool* pool, int32_t seq, int32_t index, int32_t* move_out);
+int32_t b200kv_block_pool_plan_compact(b200kv_block_pool* pool, int32_t max_moves, int32_t* moves_out);
+int32_t b200kv_block_pool_apply_moves(b200kv_block_pool* pool, const int32_t* moves, int32_t n_moves);
+int32_t b200kv_block_pool_ref_count(const b200kv_block_pool* pool, int32_t block); /* table entries that name it, -1: no such block */
 int32_t b200kv_block_pool_free_count(const b200kv_block_pool* pool);
 int32_t b200kv_block_pool_seq_len(const b200kv_block_pool* pool, int32_t seq);
 /* Host views: table [max_seqs][max_blocks_per_seq] (unused entries 0), lens [max_seqs]. */
@@ -475,7 +492,7 @@ const int32_t* b200kv_block_pool_table(const b200kv_block_pool* pool);
 const int32_t* b200kv_block_pool_lens(const b200kv_block_pool* pool);
 /* Free list in queue order; returns the count written (<= capacity). */
 int32_t b200kv_block_pool_export_free(const b200kv_block_pool* pool, int32_t* out, int32_t capacity);
-/* O(blocks) invariant check; 0 when every block is owned exactly once, else B200KV_ERR_INVALID. */
+/* O(blocks) invariant check; 0 when every block is free or held by as many sequences as are counted, else B200KV_ERR_INVALID. */
 int32_t b200kv_block_pool_validate(const b200kv_block_pool* pool);
 
 /*
@@ -583,12 +600,21 @@ int32_t b200kv_kv_cache_layer_view(const b200kv_arena* arena, const b200kv_kv_ca
  *                 to the device with ONE copy (the reference's slot mailbox, :515-519).
  *   layer_append  stages 6-8 of the reference's layer (kv_a_norm, rope, kv_cache_write) for the step's new tokens,
  *                 rows in step order (all tokens of seqs[0], then seqs[1], ...): b200kv_append_fused.
- *   layer_attend  stage 9 (decode attention of the step's sequences over their whole context) and, when out_fp8
- *                 is given, stage 10 (MX quantisation of the output): decode steps only.
+ *   layer_attend  stage 9 (attention of the step's new tokens, each over its sequence up to itself) and, when out_fp8
+ *                 is given, stage 10 (MX quantisation of the output). q and out have a row per new token, in step order.
+ *                 Several tokens of a sequence, and neighbours in `seqs` that share enough blocks, go through
+ *                 b200kv_mla_decode_shared, everything else through b200kv_mla_decode.
+ *   fork          `dst` begins as the first n_tokens of `src` (-1: all) and shares its whole blocks; the half-filled one
+ *                 is copied in every layer. Forked sequences are best kept neighbours in `seqs`.
+ *   trim          takes back the last n_tokens of a sequence (rejected drafts); a block that others hold and that is
+ *                 half filled afterwards is copied first.
+ *   compact       moves up to max_moves blocks towards the pool's start (-1: all that stand behind a free one);
+ *                 returns how many, or a negated error code. fork, trim and compact happen between steps, on the stream of
+ *                 the steps before and after; a call that fails changes nothing.
  *   abort_step    a step one of whose launches failed is taken back as a whole.
  *   end_step      the step made no allocation (the reference asserts this per step, :502-503, 535-536) and the
  *                 block pool's invariants hold.
- * Tensors are device pointers, bf16, strides in elements; q is [n_seqs][64][576] with its rope part already
+ * Tensors are device pointers, bf16, strides in elements; q is [new tokens][64][576] with its rope part already
  * rotated or rotated in place by layer_append (q_rope). The status word lives in the arena.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct b200kv_engine b200kv_engine;
@@ -621,6 +647,9 @@ int32_t b200kv_engine_layer_append(b200kv_engine* engine, int32_t layer, const v
 int32_t b200kv_engine_layer_attend(b200kv_engine* engine, int32_t layer, const void* q, int64_t q_seq_stride,
                                    int64_t q_head_stride, void* out, void* out_fp8, void* out_scales, void* stream);
 int32_t b200kv_engine_end_step(b200kv_engine* engine);
+int32_t b200kv_engine_fork(b200kv_engine* engine, int32_t src, int32_t dst, int32_t n_tokens, void* stream);
+int32_t b200kv_engine_trim(b200kv_engine* engine, int32_t seq, int32_t n_tokens, void* stream);
+int32_t b200kv_engine_compact(b200kv_engine* engine, int32_t max_moves, void* stream);
 /* Abandons the step in flight (a launch of it failed): every sequence gives back what the step added, tables,
  * lengths and the free list are as before begin_step. */
 int32_t b200kv_engine_abort_step(b200kv_engine* engine);
