@@ -615,7 +615,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (theirs != 0) {
             ok = WarpWait(bar(&misc->peer_p_full), g & 1, misc, p.status, 29);
             if (!ok) break;
-            if (ptx::ElectOne()) ptx::MbarArriveRemote(peer_p_sent);
+            if (ptx::ElectOne()) ptx::MbarArriveRemoteRelaxed(peer_p_sent);
             ok = WarpWait(bar(&misc->w_full), g & 1, misc, p.status, 28);
             if (!ok) break;
             ptx::TcFenceAfterSync();

@@ -375,9 +375,10 @@ __device__ __forceinline__ void StClusterV4(uint32_t addr, uint32_t x, uint32_t 
 __device__ __forceinline__ void LdShared128(uint32_t addr, uint32_t& x, uint32_t& y, uint32_t& z, uint32_t& w) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(w) : "r"(addr) : "memory");
 }
-// Arrival on another CTA's mbarrier (an address in the cluster's shared window).
-__device__ __forceinline__ void MbarArriveRemote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrival on another CTA's mbarrier (an address in the cluster's shared window). It orders nothing: a signal that something has
+// been seen. (With release semantics at cluster scope the thread stands still for some 1,000 cycles.)
+__device__ __forceinline__ void MbarArriveRemoteRelaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // One 4-byte store into another CTA's shared memory that completes 4 bytes on that CTA's mbarrier.
 __device__ __forceinline__ void StAsyncF32(uint32_t addr, float v, uint32_t bar) {
