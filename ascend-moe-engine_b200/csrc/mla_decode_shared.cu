@@ -67,6 +67,8 @@ constexpr int kPBytes = kRows * 128;
 constexpr int kOffPeerP = kOffP + kPBytes;                    // weights of the other CTA's tokens
 constexpr int kOffMisc = kOffPeerP + kPBytes;
 constexpr int kMiscBytes = 4096;
+// The first item's first three slabs of Q for tensor memory lie where V's second set and W will be.
+__host__ __device__ constexpr int StageOffset(int slab) { return slab < 2 ? kOffV + kVSlabs * kSlabBytes + slab * kQSlab : kOffW; }
 constexpr int kSmemBytes = kOffMisc + kMiscBytes + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 
@@ -88,6 +90,7 @@ struct Misc {
   uint64_t w_full, w_empty;    // w_empty: PV of the step is complete
   uint64_t q_full, q_empty;    // the slabs in shared memory
   uint64_t qt_full;            // the slabs in tensor memory
+  uint64_t stage_full, stage_empty;  // the first item's slabs on their way there, in buffers that no tile has yet
   uint64_t s_full, s_empty;
   uint64_t p_full;             // own weights written, rows behind the end zeroed
   uint64_t peer_p_full;        // the other CTA's weights have landed
@@ -220,13 +223,13 @@ __device__ __forceinline__ Step StepAt(const Item& it, int s) {
   return st;
 }
 
-// The cut: a step costs 2, entering another item in mid-run 6 more (Q is loaded anew and the accumulators are drained). Step x
-// of the flat list, of the item with ordinal s, stands at cost position 2x + 6s; run c takes the positions
+// The cut: a step costs 2, entering another item in mid-run 8 more (Q is loaded anew and the accumulators are drained). Step x
+// of the flat list, of the item with ordinal s, stands at cost position 2x + 8s; run c takes the positions
 // [ceil(c C / G), ceil((c + 1) C / G)).
 struct Cut {
   long long total_cost;
   long long runs;
-  static constexpr long long kStepCost = 2, kEnterCost = 6;
+  static constexpr long long kStepCost = 2, kEnterCost = 8;
   __device__ static long long Pos(long long x, long long s) { return kStepCost * x + kEnterCost * s; }
   // Non-negative quotient; the 32-bit division is several times shorter and covers every realistic size.
   __device__ static long long Div(long long a, long long b) {
@@ -296,6 +299,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::MbarInit(bar(&misc->q_full), 1);
     ptx::MbarInit(bar(&misc->q_empty), 1);
     ptx::MbarInit(bar(&misc->qt_full), kSoftmaxWarps);
+    ptx::MbarInit(bar(&misc->stage_full), 1);
+    ptx::MbarInit(bar(&misc->stage_empty), kSoftmaxWarps);
     ptx::MbarInit(bar(&misc->s_full), 1);
     ptx::MbarInit(bar(&misc->s_empty), kSoftmaxWarps);
     ptx::MbarInit(bar(&misc->p_full), kSoftmaxWarps);
@@ -411,7 +416,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::TcFenceBeforeSync();
   any_empty = __syncthreads_or(any_empty) != 0;
   ptx::TcFenceAfterSync();
-  ptx::ClusterWait();
   if (threadIdx.x == 0 && rank == 0 && p.merges_by_query == 0) p.merges[run] = make_int4(-1, -1, 0, 0);
   if (any_empty) {  // queries that attend over nothing, alone or with one like them
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
@@ -467,6 +471,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!is_w) {
         if (seg > 0) ok = WarpWait(bar(&misc->q_empty), (seg - 1) & 1, misc, p.status, 11);
         if (!ok) break;
+        // The column of slab k of Q's part in tensor memory.
+        auto q_column = [&](int k) { return 64 * (k < 2 ? kVSlabs * (1 - rank) + k : kVSlabs * rank + k - 2); };
+        if (seg == 0 && lane < 6) {
+          const int slab = lane >> 1, which = lane & 1;
+          const int query = which == 0 ? item.q0 : item.q1;
+          if (lane == 0) ptx::MbarArriveExpectTx(bar(&misc->stage_full), 3 * kQSlabBytes * (item.q1 >= 0 ? 2 : 1));
+          if (query >= 0) ptx::TmaLoad3D(base + StageOffset(slab) + which * kQSlabBytes, &q_map, q_column(slab), 0, query, bar(&misc->stage_full));
+        }
+        __syncwarp();
         if (lane < 2 * kQSmemSlabs) {  // Q's slabs in shared memory: T2, T3, rope; a box of 64 heads each for both queries
           const int slab = lane >> 1, which = lane & 1;
           const int query = which == 0 ? item.q0 : item.q1;
@@ -483,12 +496,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int32_t row = tile_row(StepAt(item, s), is_w ? 1 - rank : rank);
         const int set = g & 1;
         const uint32_t full = is_t ? bar(&misc->t_full) : is_w ? bar(&misc->w_full) : bar(&misc->v_full[set]);
-        const uint32_t empty = is_t ? bar(&misc->t_empty) : is_w ? bar(&misc->w_empty) : bar(&misc->v_empty[set]);
+        uint32_t empty = is_t ? bar(&misc->t_empty) : is_w ? bar(&misc->w_empty) : bar(&misc->v_empty[set]);
         const uint32_t dst = dst0 + (!is_t && !is_w ? set * kVSlabs * kSlabBytes : 0);
-        // Phase of the buffer's last use: T and W are used every step, a V set every other.
+        // Phase of the buffer's last use: T and W are used every step, a V set every other. W and V's second set begin as the way
+        // of Q's first slabs.
         const bool every = is_t || is_w;
-        const bool first_use = every ? g < 1 : g < 2;
-        const uint32_t parity = every ? (g & 1) ^ 1 : ((g >> 1) & 1) ^ 1;
+        const bool staged = is_w ? g == 0 : !is_t && g == 1;
+        const bool first_use = is_t ? g == 0 : !is_w && g == 0;
+        uint32_t parity = every ? (g & 1) ^ 1 : ((g >> 1) & 1) ^ 1;
+        if (staged) {
+          empty = bar(&misc->stage_empty);
+          parity = 0;
+        }
         // The warp polls together; a lane issues its slab the moment its buffer has been given back.
         bool done = !loader;
         uint64_t start = 0;
@@ -535,23 +554,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int n = __shfl_sync(0xffffffffu, hi - lo, 0);
       for (int i = 0; i < n && ok; ++i, ++g) {
         if (i == 0) {
-          ok = WarpWait(bar(&misc->q_full), seg & 1, misc, p.status, 22) && WarpWait(bar(&misc->qt_full), seg & 1, misc, p.status, 23);
+          ok = WarpWait(bar(&misc->q_full), seg & 1, misc, p.status, 22);
         }
         if (ok && g > 0) ok = WarpWait(bar(&misc->s_empty), (g & 1) ^ 1, misc, p.status, 25);
         if (ok) ok = WarpWait(bar(&misc->t_full), g & 1, misc, p.status, 24);
         if (!ok) break;
         ptx::TcFenceAfterSync();
 #pragma unroll
-        for (int k = 0; k < 4 * kTSlabs; ++k) {
+        for (int k = 8; k < 4 * kTSlabs; ++k) {  // T2 and on, whose Q lies in shared memory
           const int slab = k >> 2, kk = k & 3;
-          const uint64_t b = DescAt(t_desc, slab * kSlabBytes + kk * 32);
-          if (ptx::ElectOne()) {
-            if (slab < 2) {
-              ptx::MmaF16TS(d, tmem_u + kColQ + slab * 32 + kk * 8, b, kIdesc, k > 0 ? 1u : 0u);
-            } else {
-              ptx::MmaF16SS(d, DescAt(q_desc, (slab - 2) * kQSlab + kk * 32), b, kIdesc, 1u);
-            }
-          }
+          if (ptx::ElectOne()) ptx::MmaF16SS(d, DescAt(q_desc, (slab - 2) * kQSlab + kk * 32), DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, k > 8 ? 1u : 0u);
+        }
+        if (i == 0) ok = WarpWait(bar(&misc->qt_full), seg & 1, misc, p.status, 23);
+        if (!ok) break;
+        ptx::TcFenceAfterSync();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int slab = k >> 2, kk = k & 3;
+          if (ptx::ElectOne()) ptx::MmaF16TS(d, tmem_u + kColQ + slab * 32 + kk * 8, DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
         }
         if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty));
         const int set = __shfl_sync(0xffffffffu, g & 1, 0);
@@ -589,6 +609,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint64_t v_desc0 = ptx::SmemDescSw128(base + kOffV, kSlabBytes, 1024);  // MN-major B: next 64 columns a slab further
     const uint64_t w_desc = DescAt(v_desc0, kOffW - kOffV);
     const uint32_t peer_p_sent = ptx::MapToRank(bar(&misc->p_sent), rank ^ 1);
+    ptx::ClusterWait();  // (the peer's barriers are touched from here on)
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
     Walk walk(p, misc);
     Item item;
@@ -682,13 +703,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int x = 0;  // exchanges with the peer
     // Sends a value to the peer's thread of the same row and returns that thread's. Slots and barriers alternate: the peer
     // sends its value of exchange x + 2 only after this thread's of x + 1, which this thread sends after it has read x.
-    auto exchange = [&](float v) -> float {
+    auto send = [&](float v) {
       const int slot = x & 1;
-      const uint32_t mine = bar(&misc->max_full[slot][warp]);
-      if (lane == 0) ptx::MbarArriveExpectTx(mine, 32 * 4);
+      if (lane == 0) ptx::MbarArriveExpectTx(bar(&misc->max_full[slot][warp]), 32 * 4);
       __syncwarp();
       ptx::StAsyncF32(peer_max_at + slot * kRows * 4, v, peer_max_bar + slot * kSoftmaxWarps * 8);
-      ok = WarpWait(mine, (x >> 1) & 1, misc, p.status, 33) && ok;
+    };
+    auto receive = [&]() -> float {
+      const int slot = x & 1;
+      ok = WarpWait(bar(&misc->max_full[slot][warp]), (x >> 1) & 1, misc, p.status, 33) && ok;
       ++x;
       return *reinterpret_cast<volatile float*>(&misc->peer_max[slot][row]);
     };
@@ -701,12 +724,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // An item's rows of Q into tensor memory: T0, T1, V0-V3. A row is a lane there, and a warp reads four rows' 128 bytes with one
     // instruction, so they change places in the warp's part of the weights' buffer. The item before has had its last S, so no MMA
     // reads the old ones.
-    auto load_q = [&](const Item& it) {
+    auto load_q = [&](const Item& it, bool staged) {
       const int query = which == 0 ? it.q0 : it.q1;  // (the same for the whole warp)
       const int sub = lane >> 3, chunk = lane & 7;
       const __nv_bfloat16* q_rows = p.q + static_cast<int64_t>(query) * p.q_seq_stride + static_cast<int64_t>((warp & 1) * 32 + sub) * p.q_head_stride + 8 * chunk;
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
+      for (int half = staged ? 1 : 0; half < 2; ++half) {
         int4 v[3][8];
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
@@ -718,7 +741,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (query >= 0) v[k][i] = *reinterpret_cast<const int4*>(q_rows + static_cast<int64_t>(4 * i) * p.q_head_stride + at);
           }
         }
-        if (half == 0) weights_free();
+        if (staged) {  // the first three slabs have come by another way
+          ok = WarpWait(bar(&misc->stage_full), 0, misc, p.status, 44) && ok;
+#pragma unroll 1
+          for (int k = 0; k < 3; ++k) {
+            uint32_t r[32];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              ptx::LdShared128(base + StageOffset(k) + row * 128 + ((c ^ (row & 7)) << 4), r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+            }
+            ptx::TmemSt32(tmem + lane_base + kColQ + k * 32, r);
+          }
+          ptx::FenceProxyAsyncShared();
+          __syncwarp();
+          if (lane == 0) ptx::MbarArrive(bar(&misc->stage_empty));
+        } else if (half == 0) {
+          weights_free();
+        }
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
           __syncwarp();
@@ -745,10 +784,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       Item next_item;
       int next_lo, next_hi;
       const bool more = walk.Next(&next_item, &next_lo, &next_hi);
-      if (more) load_q(next_item);
+      if (more) load_q(next_item, !have);
+      if (!have) ptx::ClusterWait();  // (the peer's barriers are touched from here on)
       if (have) {
         // ---- epilogue of the item ----
-        const float l_all = l_run + exchange(l_run);
+        send(l_run);
+        const float l_all = l_run + receive();
         ok = WarpWait(bar(&misc->w_empty), (g & 1) ^ 1, misc, p.status, 32) && ok;
         weights_free();
         if (!ok) break;
@@ -853,24 +894,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 8; c < kTile; ++c) top[c & 7] = fmaxf(top[c & 7], f[c >> 5][c & 31]);
         float tile_max = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
-        tile_max = fmaxf(tile_max, exchange(tile_max)) * p.scale_log2;
+        send(tile_max);
+        // The weights with the reference there is, while the peer's maximum is on its way; again if that makes it move. (With no
+        // reference yet, or one that this tile alone moves, the first round would be in vain.)
+        uint32_t packed[32];
+        float sum = 0.0f;
+        auto weigh = [&](float neg_m) {
+          float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float p0 = ptx::Ex2Approx(fmaf(f[c >> 4][2 * (c & 15)], p.scale_log2, neg_m));
+            const float p1 = ptx::Ex2Approx(fmaf(f[c >> 4][2 * (c & 15) + 1], p.scale_log2, neg_m));
+            const __nv_bfloat162 pb = __floats2bfloat162_rn(p0, p1);
+            packed[c] = *reinterpret_cast<const uint32_t*>(&pb);
+            part[c & 7] += p0 + p1;
+          }
+          sum = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+        };
+        bool again = __any_sync(0xffffffffu, m_run == kLowest || tile_max * p.scale_log2 > m_run + kRescaleThreshold);
+        if (!again) weigh(-m_run);
+        tile_max = fmaxf(tile_max, receive()) * p.scale_log2;
         const bool moves = tile_max > m_run + kRescaleThreshold;
         const bool rescale = moves && m_run != kLowest;
         const float m_new = moves ? tile_max : m_run;
         const float factor = rescale ? ptx::Ex2Approx(m_run - m_new) : 1.0f;
         m_run = m_new;
-        l_run *= factor;
-        uint32_t packed[32];
-        float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float p0 = ptx::Ex2Approx(fmaf(f[c >> 4][2 * (c & 15)], p.scale_log2, -m_run));
-          const float p1 = ptx::Ex2Approx(fmaf(f[c >> 4][2 * (c & 15) + 1], p.scale_log2, -m_run));
-          const __nv_bfloat162 pb = __floats2bfloat162_rn(p0, p1);
-          packed[c] = *reinterpret_cast<const uint32_t*>(&pb);
-          part[c & 7] += p0 + p1;
-        }
-        l_run += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+        again |= __any_sync(0xffffffffu, moves) != 0;
+        if (again) weigh(-m_run);
+        l_run = l_run * factor + sum;
 
         weights_free();
         if (__any_sync(0xffffffffu, rescale)) {
@@ -922,6 +973,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   }
 
+  if (warp == 4 || warp == 5 || warp == 7) ptx::ClusterWait();
   // ---- teardown: the peer may still write into this CTA's shared memory until it has come here too ------------------
   __syncthreads();
   if (Aborting(misc)) {
