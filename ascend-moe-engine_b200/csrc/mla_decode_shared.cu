@@ -996,37 +996,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 constexpr int kMergeParts = 128;  // more than runs there are
 constexpr int kMergeRows = 32;
 
-// kStrips strips of kParts parts are in flight at a time: eight loads a thread, whatever the number of parts.
+// kStrips strips of kParts parts are in flight at a time: eight loads a thread, whatever the number of parts. The first eight are
+// the caller's, on their way while it works out the weights.
+struct MergeData {
+  const float4* at;   // this thread's row and first quad in slot 0
+  int first, parts;
+  // Part r is run (first + r)'s, in the slot of the item that it begins (the first) or continues.
+  __device__ __forceinline__ float4 Load(int strip, int r) const {
+    return at[static_cast<int64_t>(2 * (first + r) + (r == 0 ? 1 : 0)) * (kLatent / 4 * kRows) + strip * (4 * kRows)];
+  }
+};
 template <int kAllStrips, int kStrips, int kParts>
-__device__ __forceinline__ void MergeStrips(const float4* data, const int64_t (&strip)[2], int first, int parts, const float* weight, float inv,
-                                            __nv_bfloat16* out) {
+__device__ __forceinline__ void MergeStrips(const MergeData& data, float4 (&d)[8], const float* weight, float inv, __nv_bfloat16* out) {
+  static_assert(kStrips * kParts == 8);
 #pragma unroll 1
   for (int s0 = 0; s0 < kAllStrips; s0 += kStrips) {
     float4 acc[kStrips];
 #pragma unroll
     for (int s = 0; s < kStrips; ++s) acc[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-    for (int r0 = 0; r0 < parts; r0 += kParts) {
-      float4 d[kStrips][kParts];
+    for (int r0 = 0; r0 < data.parts; r0 += kParts) {
+      if (s0 + r0 > 0) {
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) {
-#pragma unroll
-        for (int s = 0; s < kStrips; ++s) {
-          // Part r is run (first + r)'s, in the slot of the item that it begins (the first) or continues.
-          if (r0 + k < parts) d[s][k] = data[(2 * (first + r0 + k) + (r0 + k == 0 ? 1 : 0)) * strip[0] + (s0 + s) * strip[1]];
+        for (int e = 0; e < 8; ++e) {
+          if (r0 + e % kParts < data.parts) d[e] = data.Load(s0 + e / kParts, r0 + e % kParts);
         }
       }
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) {
-        const float w = r0 + k < parts ? weight[(r0 + k) * kMergeRows] : 0.0f;
+      for (int e = 0; e < 8; ++e) {
+        const float w = r0 + e % kParts < data.parts ? weight[(r0 + e % kParts) * kMergeRows] : 0.0f;
         if (w == 0.0f) continue;  // no weight, and the accumulator may hold anything
-#pragma unroll
-        for (int s = 0; s < kStrips; ++s) {
-          acc[s].x = fmaf(d[s][k].x, w, acc[s].x);
-          acc[s].y = fmaf(d[s][k].y, w, acc[s].y);
-          acc[s].z = fmaf(d[s][k].z, w, acc[s].z);
-          acc[s].w = fmaf(d[s][k].w, w, acc[s].w);
-        }
+        float4& a = acc[e / kParts];
+        a.x = fmaf(d[e].x, w, a.x);
+        a.y = fmaf(d[e].y, w, a.y);
+        a.z = fmaf(d[e].z, w, a.z);
+        a.w = fmaf(d[e].w, w, a.w);
       }
     }
 #pragma unroll
@@ -1051,6 +1055,16 @@ __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constan
   const int query = rows < kHeads ? merge.x : merge.y;
   if (merge.x < 0 || query < 0) return;
   const int first = merge.z, parts = merge.w - first + 1;
+  constexpr int kStrips = kColumns / 32;
+  const int mine = 8 * (warp & 3) + (lane & 7);                               // this thread's row of the 32
+  const int quad = columns / 4 + (warp >> 2) * (kColumns / 8) + (lane >> 3);  // and its first quad of columns
+  const MergeData data{p.ws_o + static_cast<int64_t>(quad) * kRows + rows + mine, first, parts};
+  const int width = kStrips >= 4 && parts <= 2 ? 2 : kStrips >= 2 && parts <= 4 ? 4 : 8;  // parts in flight
+  float4 d[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if ((e & (width - 1)) < parts) d[e] = data.Load(width == 2 ? e >> 1 : width == 4 ? e >> 2 : 0, e & (width - 1));
+  }
   float l;
   {
     // Warp w takes parts w, w + 8, ..; a lane has a row.
@@ -1090,22 +1104,17 @@ __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constan
           l == 0.0f ? -INFINITY : static_cast<float>(static_cast<double>(m) * p.natural + static_cast<double>(logf(l)));
     }
   }
-  const int mine = 8 * (warp & 3) + (lane & 7);                                      // this thread's row of the 32
-  const int quad = columns / 4 + (warp >> 2) * (kColumns / 8) + (lane >> 3);    // and its first quad of columns
   l = __shfl_sync(0xffffffffu, l, mine);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const float4* data = p.ws_o + static_cast<int64_t>(quad) * kRows + rows + mine;
-  const int64_t strip[2] = {static_cast<int64_t>(kLatent / 4) * kRows, 4 * kRows};  // from slot to slot, from strip to strip
   __nv_bfloat16* out = p.out + (static_cast<int64_t>(query) * kHeads + ((rows + mine) & (kHeads - 1))) * kLatent + 4 * quad;
   const float* weight = &s_w[0][mine];
-  constexpr int kStrips = kColumns / 32;
-  if (kStrips >= 4 && parts <= 2) {
-    MergeStrips<kStrips, kStrips >= 4 ? 4 : 1, 2>(data, strip, first, parts, weight, inv, out);
-  } else if (kStrips >= 2 && parts <= 4) {
-    MergeStrips<kStrips, kStrips >= 2 ? 2 : 1, 4>(data, strip, first, parts, weight, inv, out);
-  } else {
-    MergeStrips<kStrips, 1, 8>(data, strip, first, parts, weight, inv, out);
+  if constexpr (kStrips >= 4) {
+    if (width == 2) return MergeStrips<kStrips, 4, 2>(data, d, weight, inv, out);
   }
+  if constexpr (kStrips >= 2) {
+    if (width == 4) return MergeStrips<kStrips, 2, 4>(data, d, weight, inv, out);
+  }
+  MergeStrips<kStrips, 1, 8>(data, d, weight, inv, out);
 }
 
 int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2 < kMergeParts ? CurrentDeviceSmCount() / 2 : kMergeParts; }
