@@ -71,8 +71,14 @@ struct b200kv_engine {
 
 namespace {
 
-// Common tokens of neighbours from which attention goes through the entry point for shared rows (a quarter of all tokens as well).
-constexpr int64_t kLeastCommon = 16384;
+// From how many common tokens (counted once a pair of neighbours) for each sequence of the step, and from what part of all tokens
+// on, attention goes through the entry point for shared rows. Both sides measured (us a layer, b200kv_mla_decode -> _shared; all
+// sequences share the given length and have 100 tokens of their own): 2 x 512 12.3 -> 12.9, 2 x 2,048 17.2 -> 14.9, 2 x 8,192
+// 22.8 -> 19.0, 4 x 1,024 14.2 -> 15.3, 4 x 4,096 19.6 -> 18.3, 8 x 1,024 17.5 -> 17.4, 8 x 2,048 18.4 -> 19.0, 8 x 8,192 28.5 -> 25.7,
+// 16 x 512 16.0 -> 17.7, 16 x 2,048 21.7 -> 20.9, 16 x 8,192 39.3 -> 31.1, 32 x 512 17.7 -> 20.4, 32 x 2,048 28.4 -> 26.3, 32 x 8,192
+// 61.6 -> 45.7, 32 x 32,768 199 -> 124.
+constexpr int64_t kLeastCommon = 1024;
+constexpr int64_t kCommonPart = 4;
 
 int32_t Refuse(const char* text) {
   SetLastError("%s", text);
@@ -125,7 +131,7 @@ bool PlanQueries(b200kv_engine* e, int32_t n_seqs, int32_t n_tokens) {
     common += shared[i];
     i += 2;
   }
-  return common >= kLeastCommon && 4 * common >= all;
+  return common >= kLeastCommon * n_seqs && kCommonPart * common >= all;
 }
 
 // Moves of blocks (pool ids) in every layer, enqueued on the stream.

@@ -402,9 +402,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         total = before;
         total_items = before_items;
         const long long cost = Cut::Pos(total, total_items > 0 ? total_items - 1 : 0);
-        // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty.
-        cut = Cut{cost, min(static_cast<long long>(runs), max(1ll, cost / Cut::kStepCost))};
-        if (p.batch > kListed) GridDependencyWait();  // (the workspace may be the preceding kernel's too)
+        // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty. And no
+        // more than pays: r runs take a step's 1.7 us times steps / r, and their parts cost the merge some 0.13 us times r / items
+        // (two queries of 16,384 tokens: 41 runs 23.5 us, all 74 of them 28.4; from 8 queries of 8,192 on it is all of them).
+        const long long paying = static_cast<long long>(sqrtf(13.0f * static_cast<float>(total) * static_cast<float>(total_items)));
+        cut = Cut{cost, max(1ll, min(static_cast<long long>(runs), min(cost / Cut::kStepCost, paying)))};
         k_lo = run < cut.runs ? cut.First(run) : cost;
         k_hi = run < cut.runs ? cut.First(run + 1) : cost;
         if (threadIdx.x == 0) misc->flat_lo = misc->flat_hi = total;
@@ -992,7 +994,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // Merges what the runs left of every item that was cut. A CTA takes 32 rows x kColumns columns of one. A warp has eight rows x four
 // quads of columns: it reads 128 bytes of a quad's rows and writes 32 bytes of a row, and goes over the strips of 16 columns of its
-// half of the CTA's columns. The rows' weights are worked out once, by the whole CTA.
+// half of the CTA's columns; with 16 columns a CTA the two halves of the warps share the parts out instead (an item of few queries
+// and many parts: 66 parts of one took 17 us with 32 columns a CTA). The rows' weights are worked out once, by the whole CTA.
 constexpr int kMergeParts = 128;  // more than runs there are
 constexpr int kMergeRows = 32;
 
@@ -1000,14 +1003,14 @@ constexpr int kMergeRows = 32;
 // the caller's, on their way while it works out the weights.
 struct MergeData {
   const float4* at;   // this thread's row and first quad in slot 0
-  int first, parts;
+  int first, begin, parts;  // the parts begin .. parts - 1 are this thread's
   // Part r is run (first + r)'s, in the slot of the item that it begins (the first) or continues.
   __device__ __forceinline__ float4 Load(int strip, int r) const {
     return at[static_cast<int64_t>(2 * (first + r) + (r == 0 ? 1 : 0)) * (kLatent / 4 * kRows) + strip * (4 * kRows)];
   }
 };
-template <int kAllStrips, int kStrips, int kParts>
-__device__ __forceinline__ void MergeStrips(const MergeData& data, float4 (&d)[8], const float* weight, float inv, __nv_bfloat16* out) {
+template <int kAllStrips, int kStrips, int kParts, bool kSplit>
+__device__ __forceinline__ void MergeStrips(const MergeData& data, float4 (&d)[8], const float* weight, float inv, __nv_bfloat16* out, float4* other) {
   static_assert(kStrips * kParts == 8);
 #pragma unroll 1
   for (int s0 = 0; s0 < kAllStrips; s0 += kStrips) {
@@ -1015,8 +1018,8 @@ __device__ __forceinline__ void MergeStrips(const MergeData& data, float4 (&d)[8
 #pragma unroll
     for (int s = 0; s < kStrips; ++s) acc[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-    for (int r0 = 0; r0 < data.parts; r0 += kParts) {
-      if (s0 + r0 > 0) {
+    for (int r0 = data.begin; r0 < data.parts; r0 += kParts) {
+      if (s0 > 0 || r0 > data.begin) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (r0 + e % kParts < data.parts) d[e] = data.Load(s0 + e / kParts, r0 + e % kParts);
@@ -1032,6 +1035,16 @@ __device__ __forceinline__ void MergeStrips(const MergeData& data, float4 (&d)[8
         a.z = fmaf(d[e].z, w, a.z);
         a.w = fmaf(d[e].w, w, a.w);
       }
+    }
+    if constexpr (kSplit) {  // the second half of the warps hands its sums over
+      const int at = threadIdx.x & 127;
+      if (threadIdx.x >= 128) other[at] = acc[0];
+      __syncthreads();
+      if (threadIdx.x >= 128) return;
+      acc[0].x += other[at].x;
+      acc[0].y += other[at].y;
+      acc[0].z += other[at].z;
+      acc[0].w += other[at].w;
     }
 #pragma unroll
     for (int s = 0; s < kStrips; ++s) {
@@ -1049,21 +1062,25 @@ __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constan
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __shared__ float s_w[kMergeParts][kMergeRows];
   __shared__ float s_m[8][kMergeRows], s_l[8][kMergeRows];
+  __shared__ float4 s_other[kColumns == 16 ? 128 : 1];
   GridDependencyWait();
   GridDependencyTrigger();
   const int4 merge = p.merges[blockIdx.y];
   const int query = rows < kHeads ? merge.x : merge.y;
   if (merge.x < 0 || query < 0) return;
   const int first = merge.z, parts = merge.w - first + 1;
-  constexpr int kStrips = kColumns / 32;
-  const int mine = 8 * (warp & 3) + (lane & 7);                               // this thread's row of the 32
-  const int quad = columns / 4 + (warp >> 2) * (kColumns / 8) + (lane >> 3);  // and its first quad of columns
-  const MergeData data{p.ws_o + static_cast<int64_t>(quad) * kRows + rows + mine, first, parts};
+  constexpr bool kSplit = kColumns == 16;
+  constexpr int kStrips = kSplit ? 1 : kColumns / 32;
+  const int mine = 8 * (warp & 3) + (lane & 7);                                                 // this thread's row of the 32
+  const int quad = columns / 4 + (kSplit ? 0 : (warp >> 2) * (kColumns / 8)) + (lane >> 3);     // and its first quad of columns
+  const int middle = kSplit ? (parts + 1) / 2 : parts;
+  const MergeData data{p.ws_o + static_cast<int64_t>(quad) * kRows + rows + mine, first, kSplit && warp >= 4 ? middle : 0, kSplit && warp >= 4 ? parts : middle};
   const int width = kStrips >= 4 && parts <= 2 ? 2 : kStrips >= 2 && parts <= 4 ? 4 : 8;  // parts in flight
   float4 d[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if ((e & (width - 1)) < parts) d[e] = data.Load(width == 2 ? e >> 1 : width == 4 ? e >> 2 : 0, e & (width - 1));
+    const int r = data.begin + (e & (width - 1));
+    if (r < data.parts) d[e] = data.Load(width == 2 ? e >> 1 : width == 4 ? e >> 2 : 0, r);
   }
   float l;
   {
@@ -1109,12 +1126,12 @@ __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constan
   __nv_bfloat16* out = p.out + (static_cast<int64_t>(query) * kHeads + ((rows + mine) & (kHeads - 1))) * kLatent + 4 * quad;
   const float* weight = &s_w[0][mine];
   if constexpr (kStrips >= 4) {
-    if (width == 2) return MergeStrips<kStrips, 4, 2>(data, d, weight, inv, out);
+    if (width == 2) return MergeStrips<kStrips, 4, 2, false>(data, d, weight, inv, out, nullptr);
   }
   if constexpr (kStrips >= 2) {
-    if (width == 4) return MergeStrips<kStrips, 2, 4>(data, d, weight, inv, out);
+    if (width == 4) return MergeStrips<kStrips, 2, 4, false>(data, d, weight, inv, out, nullptr);
   }
-  MergeStrips<kStrips, 1, 8>(data, d, weight, inv, out);
+  MergeStrips<kStrips, 1, 8, kSplit>(data, d, weight, inv, out, s_other);
 }
 
 int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2 < kMergeParts ? CurrentDeviceSmCount() / 2 : kMergeParts; }
@@ -1183,7 +1200,8 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   auto merge = [&](auto kernel, int columns) {
     return LaunchOverlapped(kernel, dim3(static_cast<unsigned>(kRows / kMergeRows * (kLatent / columns)), merges), dim3(256), 0, stream, p);
   };
-  return CheckCuda(a.batch < 37   ? merge(MlaSharedMergeKernel<32>, 32)
+  return CheckCuda(a.batch < 5    ? merge(MlaSharedMergeKernel<16>, 16)
+                   : a.batch < 37 ? merge(MlaSharedMergeKernel<32>, 32)
                    : a.batch < 74 ? merge(MlaSharedMergeKernel<64>, 64)
                    : a.batch < 148 ? merge(MlaSharedMergeKernel<128>, 128)
                                    : merge(MlaSharedMergeKernel<256>, 256),
