@@ -204,6 +204,8 @@ def _load() -> ctypes.CDLL:
         fn.restype = c_int32
     lib.b200kv_block_pool_plan_compact.argtypes = [c_void_p, c_int32, c_void_p]
     lib.b200kv_block_pool_apply_moves.argtypes = [c_void_p, c_void_p, c_int32]
+    lib.b200kv_find_shared.restype = c_int64
+    lib.b200kv_find_shared.argtypes = [c_void_p, c_int64, c_void_p, c_int32, c_int32, c_void_p, c_void_p]
     lib.b200kv_block_pool_ref_count.restype = c_int32
     lib.b200kv_block_pool_ref_count.argtypes = [c_void_p, c_int32]
     lib.b200kv_block_pool_free_count.restype = c_int32
@@ -609,6 +611,21 @@ class BlockPool:
         out = np.empty(self.num_blocks, dtype=np.int32)
         n = lib.b200kv_block_pool_export_free(self._h, out.ctypes.data, self.num_blocks)
         return out[:n].copy()
+
+
+def find_shared(table, kv_len, block_size: int):
+    """leader and shared_len (numpy int32 [B]) for mla_decode_shared from the table rows int32 [B, columns] and lengths [B] of a step
+    of one token a sequence: neighbours two by two whose rows begin with the same blocks."""
+    import numpy as np
+
+    table, lens = np.ascontiguousarray(table, dtype=np.int32), np.ascontiguousarray(kv_len, dtype=np.int32)
+    assert table.ndim == 2 and lens.shape == (len(table),)
+    leader, shared = np.empty(len(lens), dtype=np.int32), np.empty(len(lens), dtype=np.int32)
+    common = int(lib.b200kv_find_shared(table.ctypes.data, table.shape[1], lens.ctypes.data, len(lens), block_size, leader.ctypes.data,
+                                        shared.ctypes.data))
+    if common < 0:
+        raise B200KVError(-common, last_error())
+    return leader, shared
 
 
 class KvCache(Structure):

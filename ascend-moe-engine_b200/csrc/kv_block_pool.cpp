@@ -380,6 +380,37 @@ extern "C" int32_t b200kv_block_pool_apply_moves(b200kv_block_pool* pool, const 
   return B200KV_OK;
 }
 
+// Neighbours, two by two, whose table rows begin with the same blocks. Only whole blocks of both count.
+extern "C" int64_t b200kv_find_shared(const int32_t* table, int64_t max_blocks, const int32_t* kv_len, int32_t n_seqs, int32_t block_size,
+                                      int32_t* leader_out, int32_t* shared_len_out) {
+  if (table == nullptr || kv_len == nullptr || leader_out == nullptr || shared_len_out == nullptr) {
+    SetLastError("find_shared: table, kv_len, leader_out and shared_len_out must be non-null");
+    return -B200KV_ERR_NULLPTR;
+  }
+  if (n_seqs < 0 || block_size <= 0 || max_blocks <= 0) {
+    SetLastError("find_shared refused: %d sequences, blocks of %d rows, %lld blocks a row", n_seqs, block_size, static_cast<long long>(max_blocks));
+    return -B200KV_ERR_INVALID;
+  }
+  int64_t common = 0;
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    leader_out[i] = i;
+    shared_len_out[i] = 0;
+  }
+  for (int32_t i = 0; i + 1 < n_seqs; ++i) {
+    const int32_t *a = table + i * max_blocks, *b = a + max_blocks;
+    const int64_t shorter = (kv_len[i] < kv_len[i + 1] ? kv_len[i] : kv_len[i + 1]) / block_size;
+    const int64_t most = shorter < max_blocks ? shorter : max_blocks;
+    int64_t blocks = 0;
+    while (blocks < most && a[blocks] == b[blocks]) ++blocks;
+    if (blocks == 0) continue;
+    leader_out[i + 1] = i;
+    shared_len_out[i] = shared_len_out[i + 1] = static_cast<int32_t>(blocks * block_size);
+    common += shared_len_out[i];
+    ++i;  // (the pair is done with)
+  }
+  return common;
+}
+
 extern "C" int32_t b200kv_block_pool_ref_count(const b200kv_block_pool* pool, int32_t block) {
   if (pool == nullptr || block < 0 || block >= pool->num_blocks) {
     SetLastError("ref_count: block %d outside the pool", block);

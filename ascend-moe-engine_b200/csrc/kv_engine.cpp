@@ -94,7 +94,6 @@ bool PlanQueries(b200kv_engine* e, int32_t n_seqs, int32_t n_tokens) {
   int32_t *leader = kv_len + stride, *shared = leader + stride, *index = shared + stride;
   const int32_t* table = reinterpret_cast<const int32_t*>(e->staging + e->table_off);
   const int32_t* lens = reinterpret_cast<const int32_t*>(e->staging + e->lens_off);
-  const int64_t columns = e->cfg.max_blocks_per_seq;
   if (n_tokens != n_seqs) {
     int32_t at = 0;
     for (int32_t i = 0; i < n_seqs; ++i) {
@@ -108,29 +107,13 @@ bool PlanQueries(b200kv_engine* e, int32_t n_seqs, int32_t n_tokens) {
     }
     return true;
   }
-  int64_t all = 0, common = 0;  // tokens: of all queries, and those that a pair reads once instead of twice
+  int64_t all = 0;
   for (int32_t i = 0; i < n_seqs; ++i) {
     kv_len[i] = lens[i];
     index[i] = i;
-    leader[i] = i;
-    shared[i] = 0;
     all += lens[i];
   }
-  for (int32_t i = 0; i + 1 < n_seqs;) {
-    // Pair by pair, as the kernel takes them: the two rows' common blocks, of which the new tokens' own are none.
-    const int32_t *a = table + i * columns, *b = table + (i + 1) * columns;
-    const int64_t most = (lens[i] < lens[i + 1] ? lens[i] : lens[i + 1]) / e->cfg.block_size;
-    int64_t blocks = 0;
-    while (blocks < most && a[blocks] == b[blocks]) ++blocks;
-    if (blocks == 0) {
-      ++i;
-      continue;
-    }
-    leader[i + 1] = i;
-    shared[i] = shared[i + 1] = static_cast<int32_t>(blocks * e->cfg.block_size);
-    common += shared[i];
-    i += 2;
-  }
+  const int64_t common = b200kv_find_shared(table, e->cfg.max_blocks_per_seq, lens, n_seqs, e->cfg.block_size, leader, shared);
   return common >= kLeastCommon * n_seqs && kCommonPart * common >= all;
 }
 

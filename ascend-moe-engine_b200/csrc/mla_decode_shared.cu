@@ -126,6 +126,7 @@ struct SharedParams {
   int64_t pool_rows;
   int32_t batch;
   int32_t block_size;
+  int32_t longest;  // a token more than a table row holds: a longer kv_len is cut there, at its first missing block
   int32_t stable_tables;
   float scale_log2;
   double natural;  // scale / scale_log2: from the kernels' log2 domain back to natural logarithms
@@ -183,7 +184,7 @@ __device__ __forceinline__ Item MakeItem(int q0, int q1, int len0, int len1, int
 __device__ __forceinline__ Item ItemAt(const SharedParams& p, int b, bool* second) {
   const int prev = max(b - 1, 0), next = min(b + 1, p.batch - 1);
   const int lead_prev = p.leader[prev], lead = p.leader[b], lead_next = p.leader[next];
-  const int len0 = p.kv_len[b], len1 = p.kv_len[next], shared0 = p.shared_len[b], shared1 = p.shared_len[next];
+  const int len0 = min(p.kv_len[b], p.longest), len1 = min(p.kv_len[next], p.longest), shared0 = p.shared_len[b], shared1 = p.shared_len[next];
   *second = b > 0 && lead == lead_prev && ((static_cast<unsigned>(prev) - static_cast<unsigned>(lead)) & 1u) == 0;
   const bool pair = next > b && lead == lead_next && ((static_cast<unsigned>(b) - static_cast<unsigned>(lead)) & 1u) == 0;
   return MakeItem(b, pair ? next : -1, *second ? 0 : len0, pair && !*second ? len1 : 0, shared0, shared1);
@@ -351,7 +352,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             any_empty |= n == 0 && !second;
           }
         }
-        int incl = n, incl_items = n > 0 ? 1 : 0;  // (a query has at most 2^24 + 2 steps, 256 of them fit)
+        int incl = n, incl_items = n > 0 ? 1 : 0;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
           const int up = __shfl_up_sync(0xffffffffu, incl, off);
@@ -822,40 +823,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         continued = false;
         if (query >= 0) {
 #pragma unroll 1
-          for (int c = 0; c < kHalf / 32; ++c) {
-            uint32_t o[32];
-            ptx::TmemLd32(tmem + lane_base + kColO + 32 * c, o);
+          for (int c = 0; c < kHalf / 64; ++c) {
+            uint32_t o[2][32];
+            ptx::TmemLd32(tmem + lane_base + kColO + 64 * c, o[0]);
+            ptx::TmemLd32(tmem + lane_base + kColO + 64 * c + 32, o[1]);
             ptx::TmemWaitLd();
             if (!whole) {
-              uint4* dst = reinterpret_cast<uint4*>(p.ws_o) + (static_cast<int64_t>(slot) * (kLatent / 4) + (kHalf * rank + 32 * c) / 4) * kRows + row;
+              uint4* dst = reinterpret_cast<uint4*>(p.ws_o) + (static_cast<int64_t>(slot) * (kLatent / 4) + (kHalf * rank + 64 * c) / 4) * kRows + row;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) dst[k * kRows] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+              for (int k = 0; k < 16; ++k) {
+                const int j = 4 * (k & 7);
+                dst[k * kRows] = make_uint4(o[k >> 3][j], o[k >> 3][j + 1], o[k >> 3][j + 2], o[k >> 3][j + 3]);
+              }
             } else {
-              // A lane has a row; the rows' 128 bytes (two rounds) change places in the warp's part of the weights' buffer, so that a
-              // store instruction writes four rows' and not a piece of each of 32.
+              // A lane has a row; the rows' 128 bytes change places in the warp's part of the weights' buffer, so that a store
+              // instruction writes four rows' and not a piece of each of 32.
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < 8; ++k) {
                 uint32_t two[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  const __nv_bfloat162 t = __floats2bfloat162_rn(nothing ? 0.0f : __uint_as_float(o[8 * k + 2 * e]) * inv_l,
-                                                                 nothing ? 0.0f : __uint_as_float(o[8 * k + 2 * e + 1]) * inv_l);
+                  const int j = 8 * (k & 3) + 2 * e;
+                  const __nv_bfloat162 t = __floats2bfloat162_rn(nothing ? 0.0f : __uint_as_float(o[k >> 2][j]) * inv_l,
+                                                                 nothing ? 0.0f : __uint_as_float(o[k >> 2][j + 1]) * inv_l);
                   two[e] = *reinterpret_cast<const uint32_t*>(&t);
                 }
-                ptx::StShared128(p_row + (((4 * (c & 1) + k) ^ (row & 7)) << 4), two[0], two[1], two[2], two[3]);
+                ptx::StShared128(p_row + ((k ^ (row & 7)) << 4), two[0], two[1], two[2], two[3]);
               }
-              if ((c & 1) != 0) {
-                __syncwarp();
-                const int sub = lane >> 3, chunk = lane & 7;
-                __nv_bfloat16* dst = p.out + (static_cast<int64_t>(query) * kHeads + (warp & 1) * 32 + sub) * kLatent + kHalf * rank + 64 * (c >> 1) + 8 * chunk;
+              __syncwarp();
+              const int sub = lane >> 3, chunk = lane & 7;
+              __nv_bfloat16* dst = p.out + (static_cast<int64_t>(query) * kHeads + (warp & 1) * 32 + sub) * kLatent + kHalf * rank + 64 * c + 8 * chunk;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  uint4 v;
-                  ptx::LdShared128(p_warp + (4 * i + sub) * 128 + ((chunk ^ (4 * (i & 1) + sub)) << 4), v.x, v.y, v.z, v.w);
-                  *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(4 * i) * kLatent) = v;
-                }
-                __syncwarp();
+              for (int i = 0; i < 8; ++i) {
+                uint4 v;
+                ptx::LdShared128(p_warp + (4 * i + sub) * 128 + ((chunk ^ (4 * (i & 1) + sub)) << 4), v.x, v.y, v.z, v.w);
+                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(4 * i) * kLatent) = v;
               }
+              __syncwarp();
             }
           }
         }
@@ -897,8 +901,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int c = 8; c < kTile; ++c) top[c & 7] = fmaxf(top[c & 7], f[c >> 5][c & 31]);
         float tile_max = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
         send(tile_max);
-        // The weights with the reference there is, while the peer's maximum is on its way; again if that makes it move. (With no
-        // reference yet, or one that this tile alone moves, the first round would be in vain.)
+        // The weights with the reference there is, while the peer's maximum is on its way; again if that makes it move. (With a
+        // reference that this tile alone moves, the first one above all, that round would be in vain. A row of which nothing has
+        // been seen has scores of -infinity here, whose weights are zero whatever the reference.)
         uint32_t packed[32];
         float sum = 0.0f;
         auto weigh = [&](float neg_m) {
@@ -913,7 +918,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           sum = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
         };
-        bool again = __any_sync(0xffffffffu, m_run == kLowest || tile_max * p.scale_log2 > m_run + kRescaleThreshold);
+        bool again = __any_sync(0xffffffffu, tile_max * p.scale_log2 > m_run + kRescaleThreshold);
         if (!again) weigh(-m_run);
         tile_max = fmaxf(tile_max, receive()) * p.scale_log2;
         const bool moves = tile_max > m_run + kRescaleThreshold;
@@ -1176,6 +1181,7 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   p.pool_rows = a.pool.pool_rows;
   p.batch = a.batch;
   p.block_size = a.block_size;
+  p.longest = static_cast<int32_t>(a.max_blocks < (INT32_MAX - kStep) / a.block_size ? a.max_blocks * a.block_size + 1 : INT32_MAX - kStep);
   p.stable_tables = (a.flags & B200KV_DECODE_STABLE_TABLES) != 0 ? 1 : 0;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.natural = static_cast<double>(a.scale) / static_cast<double>(p.scale_log2);

@@ -216,6 +216,19 @@ def test_a_step_of_several_tokens_or_of_forks_uploads_its_queries():
     e.end_step()
 
 
+def test_find_shared():
+    table = [[3, 4, 5, 0], [3, 4, 6, 7], [3, 4, 5, 0], [3, 9, 5, 1], [8, 9, 5, 1], [8, 9, 0, 0], [2, 9, 0, 0]]
+    lens = [12, 13, 11, 16, 16, 8, 8]
+    leader, shared = b200kv.find_shared(table, lens, 4)
+    assert leader.tolist() == [0, 0, 2, 2, 4, 4, 6] and shared.tolist() == [8, 8, 4, 4, 8, 8, 0]
+    leader, shared = b200kv.find_shared(np.zeros((2, 3)), [100, 7], 4)   # lengths beyond the table; a half-filled block does not count
+    assert leader.tolist() == [0, 0] and shared.tolist() == [4, 4]
+    leader, shared = b200kv.find_shared(np.zeros((0, 3)), [], 4)
+    assert len(leader) == 0
+    with pytest.raises(b200kv.B200KVError):
+        b200kv.find_shared(table, lens, 0)
+
+
 STREAM = type("Stream", (), {"cuda_stream": 0})
 BF16, I32 = torch.bfloat16, torch.int32
 

@@ -182,6 +182,24 @@ def test_bad_table_entries_are_recorded():
         assert call.status.tolist()[0] == b200kv.DEV_BAD_BLOCK
 
 
+def test_lengths_beyond_the_table_end_at_its_first_missing_block():
+    """Whatever stands in kv_len: the call ends, says so, and the other queries' results are theirs."""
+    for long in (2 ** 31 - 1, 2 ** 30, 129):
+        case = Case([(128, [100, 128]), (0, [128]), (0, [60])] * 60).poison_unused()
+        call = Call(case)
+        call.kv_len[2::4] = long
+        call.run()
+        torch.cuda.synchronize()
+        assert call.status.tolist()[0] == b200kv.DEV_BAD_BLOCK
+        want, _, bound, _ = case.want()
+        keep = [b for b in range(case.batch) if b % 4 != 2]
+        assert ((call.out.double().cpu() - want).abs() <= bound)[keep].all()
+    case = Case([(128, [100, 128]), (0, [0])]).poison_unused()
+    call = Call(case)
+    call.kv_len[2] = -5   # a negative length is an empty one
+    call.run().check()
+
+
 def test_arrays_that_say_nothing_sensible_still_cover_every_query():
     """Leaders that name no group: queries are paired by equal leaders of neighbours only, and each reads its own rows."""
     case = Case([(0, [100]), (0, [70]), (0, [0]), (0, [200]), (0, [300])]).poison_unused()
