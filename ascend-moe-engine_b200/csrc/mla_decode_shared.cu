@@ -329,7 +329,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // (let go only after this kernel's own wait: the merge kernel reads the lengths too)
 
   // ---- this run of the list: totals, then the first step at or after the run's first cost position and the next run's ------
-  // Two passes of the same scan over the queries, 256 at a time: the first for the totals, the second finds the run's items.
+  // Passes of the same scan over the queries, 256 at a time: the first for the totals, the second finds the run's items. A run of
+  // more than kListed takes a third, which lists them in the workspace: with stable tables only there, behind the wait, since the
+  // kernel before may still read a workspace that it shares with this call.
   bool any_empty = false;
   {
     long long total = 0, total_items = 0;
@@ -338,7 +340,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Item mine;
     int n = 0;
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
+    for (int pass = 0; pass < 3; ++pass) {
+      if (pass == 2) {
+        if (p.stable_tables != 0) GridDependencyWait();
+        if (p.batch <= kListed) break;
+        __syncthreads();
+        if (misc->end_ordinal - misc->start_ordinal <= kListed) break;
+      }
       long long before = 0, before_items = 0;
 #pragma unroll 1
       for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
@@ -374,6 +382,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           chunk += of.x;
           chunk_items += of.y;
         }
+        if (pass == 2 && n > 0) {
+          const long long s = before_items + mine_items;
+          if (s >= misc->start_ordinal && s < misc->end_ordinal) p.items[s] = mine;
+        }
         if (pass == 1 && n > 0) {
           const long long first = before + mine_before, s = before_items + mine_items;
           const long long first_pos = Cut::Pos(first, s), last_pos = Cut::Pos(first + n - 1, s);
@@ -383,8 +395,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             return x > first ? x : first;
           };
           if (last_pos >= k_lo && first_pos < k_hi) {
-            misc->items[s % kListed] = mine;  // (of more than kListed the last ones stay, and none is read)
-            if (p.batch > kListed) p.items[s] = mine;
+            misc->items[s % kListed] = mine;  // (of more than kListed none is read)
             if (s == 0 || last_before < k_lo) {
               const long long x = at_or_after(k_lo);
               misc->flat_lo = x;
@@ -414,7 +425,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   }
-  if (p.stable_tables != 0) GridDependencyWait();
   GridDependencyTrigger();
   ptx::TcFenceBeforeSync();
   any_empty = __syncthreads_or(any_empty) != 0;

@@ -251,3 +251,28 @@ def test_two_calls_give_the_same_bits():
     first, second = Call(case).run(), Call(case).run()
     torch.cuda.synchronize()
     assert torch.equal(first.out, second.out) and torch.equal(first.lse, second.lse)
+
+
+def test_runs_of_many_items_in_a_workspace_that_the_call_before_reads_too():
+    """More items a run than its own list holds (some 35), with stable tables, behind a call of another kind in the same workspace."""
+    case, times = Case([(128, [130, 140]), (64, [66, 65]), (0, [3, 3]), (0, [0])] + [(0, [1 + i]) for i in range(9)]).poison_unused(), 200
+    want, want_lse, bound, lse_bound = (t.cuda() for t in case.want())
+    n, last = case.batch, int(case.leader[-1])
+    assert last == n - 1
+    many = Call(case, stable=True)
+    many.q = many.q.repeat(times, 1, 1)
+    many.out, many.lse = many.out.repeat(times, 1, 1), many.lse.repeat(times, 1)
+    many.leader = (many.leader[None, :] + n * torch.arange(times, dtype=torch.int32, device="cuda")[:, None]).flatten().contiguous()
+    many.kv_len, many.shared, many.index = many.kv_len.repeat(times), many.shared.repeat(times), many.index.repeat(times)
+    many.ws = torch.full((b200kv.decode_shared_workspace_bytes(n * times, HEADS),), 0xFF, dtype=torch.uint8, device="cuda")
+    before = torch.full((n, HEADS, LATENT), float("nan"), dtype=torch.bfloat16, device="cuda")
+    own_rows = torch.stack([many.table[i] for i in case.table_index]).contiguous()
+    for _ in range(3):
+        b200kv.mla_decode(case.q.cuda(), many.view, own_rows, to_dev_i32(case.kv_len), case.block, case.scale, out=before,
+                          workspace=many.ws, status=many.status, stable_tables=True)
+        many.run()
+    status_ok(many.status)
+    assert ((before.double() - want).abs() <= bound).all()
+    assert ((many.out.double().view(times, n, HEADS, LATENT) - want).abs() <= bound).all()
+    lse, empty = many.lse.double().view(times, n, HEADS), torch.isinf(want_lse)
+    assert (lse[:, empty] == -float("inf")).all() and ((lse - want_lse).abs()[:, ~empty] <= lse_bound[~empty]).all()
