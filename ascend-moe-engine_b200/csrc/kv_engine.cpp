@@ -388,7 +388,9 @@ extern "C" int32_t b200kv_engine_layer_attend(b200kv_engine* e, int32_t layer, c
   if (e == nullptr) return B200KV_ERR_NULLPTR;
   if (!e->in_step) return Refuse("engine_layer_attend: no step in flight");
   if (out_fp8 != nullptr && out_scales == nullptr) return Refuse("engine_layer_attend: out_fp8 without out_scales");
-  if (e->step_shares) {
+  // (one token a sequence, and rows that only the other entry point takes: not a reason to refuse the step)
+  const bool fits = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0 && q_seq_stride % 8 == 0 && q_head_stride % 8 == 0;
+  if (e->step_shares && (fits || e->step_tokens != e->step_seqs)) {
     b200kv_shared_args a{};
     if (int32_t rc = b200kv_kv_cache_layer_view(e->arena, &e->cache, layer, &a.pool)) return rc;
     const int64_t stride = e->cfg.max_step_tokens;
