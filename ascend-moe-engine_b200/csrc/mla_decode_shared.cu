@@ -30,6 +30,8 @@
 // together through the cluster barrier.
 #include <cuda.h>
 
+#include <climits>
+
 #include "common.cuh"
 #include "mla_tc_common.cuh"
 #include "sm100_ptx.cuh"
@@ -38,7 +40,7 @@ namespace b200kv {
 
 int32_t ValidatePoolView(const b200kv_pool_view* pool);
 int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, CUtensorMap* out);
-int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, CUtensorMap* out);
+int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, int32_t slabs, CUtensorMap* out);
 int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t box_heads,
                 CUtensorMap* out);
 
@@ -67,8 +69,14 @@ constexpr int kPBytes = kRows * 128;
 constexpr int kOffPeerP = kOffP + kPBytes;                    // weights of the other CTA's tokens
 constexpr int kOffMisc = kOffPeerP + kPBytes;
 constexpr int kMiscBytes = 4096;
-// The first item's first three slabs of Q for tensor memory lie where V's second set and W will be.
-__host__ __device__ constexpr int StageOffset(int slab) { return slab < 2 ? kOffV + kVSlabs * kSlabBytes + slab * kQSlab : kOffW; }
+// An item's slabs of Q for tensor memory come two at a time, through buffers that have no tile then: V's set of the item's first
+// step, T, and V's set again; V's second set, W, and V's second set for a run's first item, whose tiles come at the same time.
+constexpr int kRounds = 3;
+static_assert(2 * kRounds == kQTmemSlabs && 2 * kQSlab <= kVSlabs * kSlabBytes);
+__device__ __forceinline__ int StageOffset(int round, int seg, int set) {
+  const int v = kOffV + (seg == 0 ? 1 : set) * kVSlabs * kSlabBytes;
+  return round != 1 ? v : seg == 0 ? kOffW : kOffT;
+}
 constexpr int kSmemBytes = kOffMisc + kMiscBytes + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 
@@ -85,12 +93,12 @@ struct Item {
 constexpr int kListed = 32;  // a run of up to so many items finds them in shared memory
 
 struct Misc {
-  uint64_t t_full, t_empty;
+  uint64_t t_full[2], t_empty[2];  // T2, T3 and the rope; T0 and T1
   uint64_t v_full[2], v_empty[2];
   uint64_t w_full, w_empty;    // w_empty: PV of the step is complete
   uint64_t q_full, q_empty;    // the slabs in shared memory
   uint64_t qt_full;            // the slabs in tensor memory
-  uint64_t stage_full, stage_empty;  // the first item's slabs on their way there, in buffers that no tile has yet
+  uint64_t stage_full[kRounds], stage_empty[kRounds];  // and on their way there
   uint64_t s_full, s_empty;
   uint64_t p_full;             // own weights written, rows behind the end zeroed
   uint64_t peer_p_full;        // the other CTA's weights have landed
@@ -106,7 +114,7 @@ struct Misc {
   int32_t began_in;    // the run that item began in
   long long start_ordinal, end_ordinal;  // the run's items
   long long flat_lo, flat_hi;
-  uint2 scan[kThreads / 32];
+  longlong2 scan[kThreads / 32];
   float peer_max[2][kRows];
   Item items[kListed];  // by ordinal % kListed; a run of more than kListed items reads SharedParams::items
 };
@@ -272,8 +280,9 @@ __device__ __forceinline__ bool WarpWait(uint32_t bar, uint32_t parity, Misc* mi
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    MlaDecodeSharedKernel(const __grid_constant__ CUtensorMap latent_map, const __grid_constant__ CUtensorMap rope_map,
-                          const __grid_constant__ CUtensorMap q_map, const __grid_constant__ SharedParams p) {
+    MlaDecodeSharedKernel(const __grid_constant__ CUtensorMap latent_map, const __grid_constant__ CUtensorMap t_map,
+                          const __grid_constant__ CUtensorMap rope_map, const __grid_constant__ CUtensorMap q_map,
+                          const __grid_constant__ SharedParams p) {
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t raw = ptx::SmemAddr(smem_dyn);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -287,9 +296,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   auto bar = [&](const uint64_t* b) { return ptx::SmemAddr(b); };
 
   if (threadIdx.x == 0) {
-    ptx::MbarInit(bar(&misc->t_full), 1);
-    ptx::MbarInit(bar(&misc->t_empty), 1);
     for (int s = 0; s < 2; ++s) {
+      ptx::MbarInit(bar(&misc->t_full[s]), 1);
+      ptx::MbarInit(bar(&misc->t_empty[s]), 1);
       ptx::MbarInit(bar(&misc->v_full[s]), 1);
       ptx::MbarInit(bar(&misc->v_empty[s]), 1);
       ptx::MbarInit(bar(&misc->drain[s]), 1);
@@ -300,8 +309,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::MbarInit(bar(&misc->q_full), 1);
     ptx::MbarInit(bar(&misc->q_empty), 1);
     ptx::MbarInit(bar(&misc->qt_full), kSoftmaxWarps);
-    ptx::MbarInit(bar(&misc->stage_full), 1);
-    ptx::MbarInit(bar(&misc->stage_empty), kSoftmaxWarps);
+    for (int r = 0; r < kRounds; ++r) {
+      ptx::MbarInit(bar(&misc->stage_full[r]), 1);
+      ptx::MbarInit(bar(&misc->stage_empty[r]), kSoftmaxWarps);
+    }
     ptx::MbarInit(bar(&misc->s_full), 1);
     ptx::MbarInit(bar(&misc->s_empty), kSoftmaxWarps);
     ptx::MbarInit(bar(&misc->p_full), kSoftmaxWarps);
@@ -314,8 +325,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     misc->start_step = 0;
     misc->began_in = 0;
     misc->start_ordinal = misc->end_ordinal = 0;
+    misc->flat_lo = LLONG_MAX;  // (a run between two items has none)
+    misc->flat_hi = 0;
     ptx::FenceBarrierInit();
     ptx::PrefetchTensorMap(&latent_map);
+    ptx::PrefetchTensorMap(&t_map);
     ptx::PrefetchTensorMap(&rope_map);
     ptx::PrefetchTensorMap(&q_map);
   }
@@ -329,99 +343,105 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // (let go only after this kernel's own wait: the merge kernel reads the lengths too)
 
   // ---- this run of the list: totals, then the first step at or after the run's first cost position and the next run's ------
-  // Passes of the same scan over the queries, 256 at a time: the first for the totals, the second finds the run's items. A run of
-  // more than kListed takes a third, which lists them in the workspace: with stable tables only there, behind the wait, since the
-  // kernel before may still read a workspace that it shares with this call.
+  // Each thread has a stretch of the queries: sums over it, one scan over the threads, and those threads that have items of this
+  // run go over their stretch again.
+  const int each = (p.batch - 1) / kThreads + 1;
+  const int stretch = min(static_cast<int>(threadIdx.x) * each, p.batch), stretch_end = min(stretch + each, p.batch);
   bool any_empty = false;
   {
-    long long total = 0, total_items = 0;
-    Cut cut{};
-    long long k_lo = 0, k_hi = 0;
     Item mine;
-    int n = 0;
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      if (pass == 2) {
-        if (p.stable_tables != 0) GridDependencyWait();
-        if (p.batch <= kListed) break;
-        __syncthreads();
-        if (misc->end_ordinal - misc->start_ordinal <= kListed) break;
-      }
-      long long before = 0, before_items = 0;
-#pragma unroll 1
-      for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-        const int b = b0 + threadIdx.x;
-        if (pass == 0 || p.batch > kThreads) {  // (a batch of one chunk keeps what it has loaded)
-          n = 0;
-          if (b < p.batch) {
-            bool second;
-            mine = ItemAt(p, b, &second);
-            n = mine.steps();
-            any_empty |= n == 0 && !second;
-          }
-        }
-        int incl = n, incl_items = n > 0 ? 1 : 0;
+    long long n = 0;
+    int n_items = 0;
+#pragma unroll 4
+    for (int b = stretch; b < stretch_end; ++b) {
+      bool second;
+      mine = ItemAt(p, b, &second);
+      const int steps = mine.steps();
+      n += steps;
+      n_items += steps > 0 ? 1 : 0;
+      any_empty |= steps == 0 && !second;
+    }
+    long long incl = n;
+    int incl_items = n_items;
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, incl, off);
-          const int up_items = __shfl_up_sync(0xffffffffu, incl_items, off);
-          if (lane >= off) {
-            incl += up;
-            incl_items += up_items;
-          }
-        }
-        __syncthreads();  // (the chunk before has been read)
-        if (lane == 31) misc->scan[warp] = make_uint2(incl, incl_items);
-        __syncthreads();
-        long long chunk = 0, chunk_items = 0, mine_before = incl - n, mine_items = incl_items - 1;
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) {
-          const uint2 of = misc->scan[w];
-          mine_before += w < warp ? of.x : 0;
-          mine_items += w < warp ? of.y : 0;
-          chunk += of.x;
-          chunk_items += of.y;
-        }
-        if (pass == 2 && n > 0) {
-          const long long s = before_items + mine_items;
-          if (s >= misc->start_ordinal && s < misc->end_ordinal) p.items[s] = mine;
-        }
-        if (pass == 1 && n > 0) {
-          const long long first = before + mine_before, s = before_items + mine_items;
-          const long long first_pos = Cut::Pos(first, s), last_pos = Cut::Pos(first + n - 1, s);
-          const long long last_before = Cut::Pos(first - 1, s - 1);  // the item before this one ends here
-          auto at_or_after = [&](long long k) {                      // first step at or after cost position k, if it is in this item
-            const long long x = (k - Cut::kEnterCost * s + 1) >> 1;
-            return x > first ? x : first;
-          };
-          if (last_pos >= k_lo && first_pos < k_hi) {
-            misc->items[s % kListed] = mine;  // (of more than kListed none is read)
-            if (s == 0 || last_before < k_lo) {
-              const long long x = at_or_after(k_lo);
-              misc->flat_lo = x;
-              misc->start_step = static_cast<int>(x - first);
-              misc->start_ordinal = s;
-              misc->began_in = static_cast<int>(cut.RunOf(first_pos));
-            }
-            atomicMax(reinterpret_cast<unsigned long long*>(&misc->end_ordinal), static_cast<unsigned long long>(s + 1));
-          }
-          if (last_pos >= k_hi && (s == 0 || last_before < k_hi)) misc->flat_hi = at_or_after(k_hi);
-        }
-        before += chunk;
-        before_items += chunk_items;
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, off);
+      const int up_items = __shfl_up_sync(0xffffffffu, incl_items, off);
+      if (lane >= off) {
+        incl += up;
+        incl_items += up_items;
       }
-      if (pass == 0) {
-        total = before;
-        total_items = before_items;
-        const long long cost = Cut::Pos(total, total_items > 0 ? total_items - 1 : 0);
-        // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty. And no
-        // more than pays: r runs take a step's 1.7 us times steps / r, and their parts cost the merge some 0.13 us times r / items
-        // (two queries of 16,384 tokens: 41 runs 23.5 us, all 74 of them 28.4; from 8 queries of 8,192 on it is all of them).
-        const long long paying = static_cast<long long>(sqrtf(13.0f * static_cast<float>(total) * static_cast<float>(total_items)));
-        cut = Cut{cost, max(1ll, min(static_cast<long long>(runs), min(cost / Cut::kStepCost, paying)))};
-        k_lo = run < cut.runs ? cut.First(run) : cost;
-        k_hi = run < cut.runs ? cut.First(run + 1) : cost;
-        if (threadIdx.x == 0) misc->flat_lo = misc->flat_hi = total;
+    }
+    if (lane == 31) misc->scan[warp] = make_longlong2(incl, incl_items);
+    __syncthreads();
+    long long total = 0, total_items = 0, before = incl - n, before_items = incl_items - n_items;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const longlong2 of = misc->scan[w];
+      before += w < warp ? of.x : 0;
+      before_items += w < warp ? of.y : 0;
+      total += of.x;
+      total_items += of.y;
+    }
+    const long long cost = Cut::Pos(total, total_items > 0 ? total_items - 1 : 0);
+    // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty. And no
+    // more than pays: r runs take a step's 1.7 us times steps / r, and their parts cost the merge some 0.13 us times r / items
+    // (two queries of 16,384 tokens: 41 runs 23.5 us, all 74 of them 28.4; from 8 queries of 8,192 on it is all of them).
+    const long long paying = static_cast<long long>(sqrtf(13.0f * static_cast<float>(total) * static_cast<float>(total_items)));
+    const Cut cut{cost, max(1ll, min(static_cast<long long>(runs), min(cost / Cut::kStepCost, paying)))};
+    const long long k_lo = run < cut.runs ? cut.First(run) : cost, k_hi = run < cut.runs ? cut.First(run + 1) : cost;
+    // The stretch's items, in order: f(item, its first step, its ordinal).
+    auto each_item = [&](auto f) {
+      long long first = before, s = before_items;
+#pragma unroll 1
+      for (int b = stretch; b < stretch_end; ++b) {
+        if (each > 1) {  // (a stretch of one is still at hand)
+          bool second;
+          mine = ItemAt(p, b, &second);
+        }
+        const int steps = mine.steps();
+        if (steps == 0) continue;
+        f(mine, first, s);
+        first += steps;
+        ++s;
+      }
+    };
+    const bool here = n_items > 0 && Cut::Pos(before + n - 1, before_items + n_items - 1) >= k_lo &&
+                      (before_items == 0 || Cut::Pos(before - 1, before_items - 1) < k_hi);
+    if (here) {
+      each_item([&](const Item& item, long long first, long long s) {
+        const long long first_pos = Cut::Pos(first, s), last_pos = Cut::Pos(first + item.steps() - 1, s);
+        const long long last_before = Cut::Pos(first - 1, s - 1);  // the item before this one ends here
+        auto at_or_after = [&](long long k) {                      // first step at or after cost position k, if it is in this item
+          const long long x = (k - Cut::kEnterCost * s + 1) >> 1;
+          return x > first ? x : first;
+        };
+        if (last_pos >= k_lo && first_pos < k_hi) {
+          misc->items[s % kListed] = item;  // (of more than kListed none is read)
+          if (s == 0 || last_before < k_lo) {
+            const long long x = at_or_after(k_lo);
+            misc->flat_lo = x;
+            misc->start_step = static_cast<int>(x - first);
+            misc->start_ordinal = s;
+            misc->began_in = static_cast<int>(cut.RunOf(first_pos));
+          }
+          atomicMax(reinterpret_cast<unsigned long long*>(&misc->end_ordinal), static_cast<unsigned long long>(s + 1));
+        }
+        if (last_pos >= k_hi && (s == 0 || last_before < k_hi)) misc->flat_hi = at_or_after(k_hi);
+      });
+    }
+    // Up to the last cost position and behind it: the end of the list.
+    if (threadIdx.x == 0 && k_lo >= cost) misc->flat_lo = total;
+    if (threadIdx.x == 0 && k_hi >= cost) misc->flat_hi = total;
+    if (p.stable_tables != 0) GridDependencyWait();
+    // A run of more than kListed items lists them in the workspace, only here, behind the wait: the kernel before may still read a
+    // workspace that it shares with this call.
+    if (p.batch > kListed) {
+      __syncthreads();
+      if (here && misc->end_ordinal - misc->start_ordinal > kListed) {
+        each_item([&](const Item& item, long long, long long s) {
+          if (s >= misc->start_ordinal && s < misc->end_ordinal) p.items[s] = item;
+        });
       }
     }
   }
@@ -448,8 +468,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 4 || warp == 7) {
     // ======================= loads ============================================================================
-    // Warp 4 brings a step's T and V (and Q), warp 7 its W, which waits for the PV before: in one warp that wait would hold the
-    // next step's T back.
+    // Warp 4 brings a step's T and V, warp 7 an item's Q and a step's W, which waits for the PV before: in one warp that wait would
+    // hold the next step's T back.
     // Pool row of a tile, through the block table; the row behind the pool (which loads as zeros) for a tile without tokens and
     // for a bad entry, which is recorded.
     auto tile_row = [&](const Step& st, int tile) -> int32_t {
@@ -467,59 +487,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       return static_cast<int32_t>(row);
     };
-    // Warp 4: lane 0 T's four latent slabs, lane 1 its rope slab, lane 2 V. Warp 7: lane 0 the other tile's slabs of V's columns.
-    // Four slabs are one box: a warp issues a load only every 170 cycles or so.
-    const bool is_w = warp == 7, is_t = !is_w && lane < 2;
-    const bool loader = lane < (is_w ? 1 : 3);
+    // Warp 4: lane 0 T2 and T3, lane 1 the rope slab, lane 2 T0 and T1, lane 3 V. Warp 7: lane 0 the other tile's slabs of V's
+    // columns. Several slabs are one box: a warp issues a load only every 170 cycles or so.
+    const bool is_w = warp == 7, is_t = !is_w && lane < 3;
+    const bool loader = lane < (is_w ? 1 : 4);
     const bool is_rope = is_t && lane == 1;
-    const int first_slab = is_t ? kVSlabs * (1 - rank) : kVSlabs * rank;
+    const int group = lane == 2 ? 1 : 0;  // of T
+    const int first_slab = is_t ? kVSlabs * (1 - rank) + (group == 0 ? 2 : 0) : kVSlabs * rank;
     const bool announces = loader && !is_rope;
-    const uint32_t announced = (is_t ? kTSlabs : kVSlabs) * kSlabBytes;
-    const uint32_t dst0 = base + (is_t ? kOffT : is_w ? kOffW : kOffV) + (is_rope ? kVSlabs * kSlabBytes : 0);
+    const uint32_t announced = (!is_t ? kVSlabs : group == 0 ? 3 : 2) * kSlabBytes;
+    const uint32_t dst0 = base + (is_t ? kOffT : is_w ? kOffW : kOffV) + (is_rope ? 4 : is_t && group == 0 ? 2 : 0) * kSlabBytes;
+    const CUtensorMap* const map = is_t ? &t_map : &latent_map;
     Walk walk(p, misc);
     Item item;
     int lo, hi;
     int g = 0, seg = 0;
     while (ok && walk.Next(&item, &lo, &hi)) {
-      if (!is_w) {
-        if (seg > 0) ok = WarpWait(bar(&misc->q_empty), (seg - 1) & 1, misc, p.status, 11);
+      // Once the item before has had its last S, Q's old slabs, T and what was staged have been read (the waits for stage_empty
+      // below take an earlier phase for the item's otherwise); V's set was the PV's before the last.
+      if (seg > 0) ok = WarpWait(bar(&misc->q_empty), (seg - 1) & 1, misc, p.status, 11);
+      if (!ok) break;
+      if (is_w) {
+        if (g > 1) ok = WarpWait(bar(&misc->v_empty[g & 1]), ((g >> 1) & 1) ^ 1, misc, p.status, 12);
         if (!ok) break;
-        // The column of slab k of Q's part in tensor memory.
-        auto q_column = [&](int k) { return 64 * (k < 2 ? kVSlabs * (1 - rank) + k : kVSlabs * rank + k - 2); };
-        if (seg == 0 && lane < 6) {
-          const int slab = lane >> 1, which = lane & 1;
-          const int query = which == 0 ? item.q0 : item.q1;
-          if (lane == 0) ptx::MbarArriveExpectTx(bar(&misc->stage_full), 3 * kQSlabBytes * (item.q1 >= 0 ? 2 : 1));
-          if (query >= 0) ptx::TmaLoad3D(base + StageOffset(slab) + which * kQSlabBytes, &q_map, q_column(slab), 0, query, bar(&misc->stage_full));
-        }
+        // A box is the 64 heads of one query: which of the two is the lane's last bit.
+        const int which = lane & 1, query = which == 0 ? item.q0 : item.q1;
+        const uint32_t slab_bytes = kQSlabBytes * (item.q1 >= 0 ? 2 : 1);
+        auto staged = [&](int round, int of_two) {
+          const int slab = 2 * round + of_two;
+          const uint32_t full = bar(&misc->stage_full[round]);
+          if (of_two == 0 && which == 0) ptx::MbarArriveExpectTx(full, 2 * slab_bytes);
+          if (query >= 0) {
+            const int x = 64 * (slab < 2 ? kVSlabs * (1 - rank) + slab : kVSlabs * rank + slab - 2);
+            ptx::TmaLoad3D(base + StageOffset(round, seg, g & 1) + of_two * kQSlab + which * kQSlabBytes, &q_map, x, 0, query, full);
+          }
+        };
+        if (lane < 8) staged(lane >> 2, (lane >> 1) & 1);
         __syncwarp();
-        if (lane < 2 * kQSmemSlabs) {  // Q's slabs in shared memory: T2, T3, rope; a box of 64 heads each for both queries
-          const int slab = lane >> 1, which = lane & 1;
-          const int query = which == 0 ? item.q0 : item.q1;
+        if (lane < 2 * kQSmemSlabs) {  // the slabs in shared memory: T2, T3, rope
+          const int slab = lane >> 1;
           const uint32_t full = bar(&misc->q_full);
-          if (lane == 0) ptx::MbarArriveExpectTx(full, kQSmemSlabs * kQSlabBytes * (item.q1 >= 0 ? 2 : 1));
+          if (lane == 0) ptx::MbarArriveExpectTx(full, kQSmemSlabs * slab_bytes);
           if (query >= 0) {
             const int x = slab == 2 ? kLatent : 64 * (kVSlabs * (1 - rank) + 2 + slab);
             ptx::TmaLoad3D(base + kOffQ + slab * kQSlab + which * kQSlabBytes, &q_map, x, 0, query, full);
           }
         }
-        ++seg;
+        __syncwarp();
+        ok = WarpWait(bar(&misc->stage_empty[0]), seg & 1, misc, p.status, 13);
+        if (!ok) break;
+        if (lane < 4) staged(2, lane >> 1);
+        __syncwarp();
       }
       for (int s = lo; s < hi; ++s, ++g) {
         const int32_t row = tile_row(StepAt(item, s), is_w ? 1 - rank : rank);
         const int set = g & 1;
-        const uint32_t full = is_t ? bar(&misc->t_full) : is_w ? bar(&misc->w_full) : bar(&misc->v_full[set]);
-        uint32_t empty = is_t ? bar(&misc->t_empty) : is_w ? bar(&misc->w_empty) : bar(&misc->v_empty[set]);
+        const uint32_t full = is_t ? bar(&misc->t_full[group]) : is_w ? bar(&misc->w_full) : bar(&misc->v_full[set]);
+        uint32_t empty = is_t ? bar(&misc->t_empty[group]) : is_w ? bar(&misc->w_empty) : bar(&misc->v_empty[set]);
         const uint32_t dst = dst0 + (!is_t && !is_w ? set * kVSlabs * kSlabBytes : 0);
-        // Phase of the buffer's last use: T and W are used every step, a V set every other. W and V's second set begin as the way
-        // of Q's first slabs.
+        // Phase of the buffer's last use: T and W are used every step, a V set every other. An item's first tiles come behind the
+        // slabs of Q that have passed through their buffers; in a run's first item these are W's first and V's second.
         const bool every = is_t || is_w;
-        const bool staged = is_w ? g == 0 : !is_t && g == 1;
-        const bool first_use = is_t ? g == 0 : !is_w && g == 0;
+        const bool first_use = g == 0 && !is_w;
         uint32_t parity = every ? (g & 1) ^ 1 : ((g >> 1) & 1) ^ 1;
-        if (staged) {
-          empty = bar(&misc->stage_empty);
-          parity = 0;
+        if (seg == 0 ? (is_w ? g == 0 : !is_t && g == 1) : s == lo && !is_w) {
+          empty = bar(&misc->stage_empty[every ? 1 : kRounds - 1]);
+          parity = seg & 1;
         }
         // The warp polls together; a lane issues its slab the moment its buffer has been given back.
         bool done = !loader;
@@ -530,7 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (is_rope) {
               ptx::TmaLoad2D(dst, &rope_map, 0, row, full);
             } else {
-              ptx::TmaLoad3D(dst, &latent_map, 0, row, first_slab, full);
+              ptx::TmaLoad3D(dst, map, 0, row, first_slab, full);
             }
             done = true;
           }
@@ -548,6 +581,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
+      ++seg;
     }
   } else if (warp == 5) {
     // ======================= QK ================================================================================
@@ -570,7 +604,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ok = WarpWait(bar(&misc->q_full), seg & 1, misc, p.status, 22);
         }
         if (ok && g > 0) ok = WarpWait(bar(&misc->s_empty), (g & 1) ^ 1, misc, p.status, 25);
-        if (ok) ok = WarpWait(bar(&misc->t_full), g & 1, misc, p.status, 24);
+        if (ok) ok = WarpWait(bar(&misc->t_full[0]), g & 1, misc, p.status, 24);
         if (!ok) break;
         ptx::TcFenceAfterSync();
 #pragma unroll
@@ -578,7 +612,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int slab = k >> 2, kk = k & 3;
           if (ptx::ElectOne()) ptx::MmaF16SS(d, DescAt(q_desc, (slab - 2) * kQSlab + kk * 32), DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, k > 8 ? 1u : 0u);
         }
-        if (i == 0) ok = WarpWait(bar(&misc->qt_full), seg & 1, misc, p.status, 23);
+        if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty[0]));
+        ok = WarpWait(bar(&misc->t_full[1]), g & 1, misc, p.status, 24);
+        if (ok && i == 0) ok = WarpWait(bar(&misc->qt_full), seg & 1, misc, p.status, 23);
         if (!ok) break;
         ptx::TcFenceAfterSync();
 #pragma unroll
@@ -586,7 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int slab = k >> 2, kk = k & 3;
           if (ptx::ElectOne()) ptx::MmaF16TS(d, tmem_u + kColQ + slab * 32 + kk * 8, DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
         }
-        if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty));
+        if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty[1]));
         const int set = __shfl_sync(0xffffffffu, g & 1, 0);
         const uint64_t v_desc = DescAt(v_desc0, set * kVSlabs * kSlabBytes);
         ok = WarpWait(bar(&misc->v_full[set]), (g >> 1) & 1, misc, p.status, 26);
@@ -734,61 +770,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = WarpWait(bar(&misc->p_empty), (g & 1) ^ 1, misc, p.status, 31) && WarpWait(bar(&misc->p_sent), (g & 1) ^ 1, misc, p.status, 38) && ok;
       }
     };
-    // An item's rows of Q into tensor memory: T0, T1, V0-V3. A row is a lane there, and a warp reads four rows' 128 bytes with one
-    // instruction, so they change places in the warp's part of the weights' buffer. The item before has had its last S, so no MMA
-    // reads the old ones.
-    auto load_q = [&](const Item& it, bool staged) {
-      const int query = which == 0 ? it.q0 : it.q1;  // (the same for the whole warp)
-      const int sub = lane >> 3, chunk = lane & 7;
-      const __nv_bfloat16* q_rows = p.q + static_cast<int64_t>(query) * p.q_seq_stride + static_cast<int64_t>((warp & 1) * 32 + sub) * p.q_head_stride + 8 * chunk;
+    // An item's rows of Q from where they have been brought into tensor memory, where a row is a lane: T0, T1, V0-V3. The item
+    // before has had its last S, so no MMA reads the old ones. (Reads of Q by the threads themselves take two to three times as
+    // long as this way through shared memory, 24 or 48 of them a thread.)
+    int seg = 0;
+    auto load_q = [&](int set) {
 #pragma unroll 1
-      for (int half = staged ? 1 : 0; half < 2; ++half) {
-        int4 v[3][8];
+      for (int round = 0; round < kRounds; ++round) {
+        ok = WarpWait(bar(&misc->stage_full[round]), seg & 1, misc, p.status, 44) && ok;
+        const uint32_t at = base + StageOffset(round, seg, set) + row * 128;
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const int slab = 3 * half + k;
-          const int at = 64 * (slab < 2 ? kVSlabs * (1 - rank) + slab : kVSlabs * rank + slab - 2);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[k][i] = make_int4(0, 0, 0, 0);
-            if (query >= 0) v[k][i] = *reinterpret_cast<const int4*>(q_rows + static_cast<int64_t>(4 * i) * p.q_head_stride + at);
-          }
-        }
-        if (staged) {  // the first three slabs have come by another way
-          ok = WarpWait(bar(&misc->stage_full), 0, misc, p.status, 44) && ok;
-#pragma unroll 1
-          for (int k = 0; k < 3; ++k) {
-            uint32_t r[32];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              ptx::LdShared128(base + StageOffset(k) + row * 128 + ((c ^ (row & 7)) << 4), r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-            }
-            ptx::TmemSt32(tmem + lane_base + kColQ + k * 32, r);
-          }
-          ptx::FenceProxyAsyncShared();
-          __syncwarp();
-          if (lane == 0) ptx::MbarArrive(bar(&misc->stage_empty));
-        } else if (half == 0) {
-          weights_free();
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {  // row 4 i + sub of the warp's 32
-            ptx::StShared128(p_warp + (4 * i + sub) * 128 + ((chunk ^ (4 * (i & 1) + sub)) << 4), v[k][i].x, v[k][i].y, v[k][i].z, v[k][i].w);
-          }
-          __syncwarp();
+        for (int k = 0; k < 2; ++k) {
           uint32_t r[32];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) ptx::LdShared128(p_row + ((c ^ (row & 7)) << 4), r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-          ptx::TmemSt32(tmem + lane_base + kColQ + (3 * half + k) * 32, r);
+          for (int c = 0; c < 8; ++c) ptx::LdShared128(at + k * kQSlab + ((c ^ (row & 7)) << 4), r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+          ptx::TmemSt32(tmem + lane_base + kColQ + (2 * round + k) * 32, r);
         }
+        ptx::FenceProxyAsyncShared();
+        __syncwarp();
+        if (lane == 0) ptx::MbarArrive(bar(&misc->stage_empty[round]));
       }
       ptx::TmemWaitSt();
       ptx::TcFenceBeforeSync();
       __syncwarp();
       if (lane == 0) ptx::MbarArrive(bar(&misc->qt_full));
+      ++seg;
     };
     bool have = false, continued = misc->start_step > 0;
     float m_run = kLowest, l_run = 0.0f;
@@ -797,7 +803,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       Item next_item;
       int next_lo, next_hi;
       const bool more = walk.Next(&next_item, &next_lo, &next_hi);
-      if (more) load_q(next_item, !have);
+      if (more) load_q(g & 1);
       if (!have) ptx::ClusterWait();  // (the peer's barriers are touched from here on)
       if (have) {
         // ---- epilogue of the item ----
@@ -1172,8 +1178,9 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
     }
     configured_device = device;
   }
-  CUtensorMap latent_map, rope_map, q_map;
-  if (int32_t rc = GetSlabMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, &latent_map)) return rc;
+  CUtensorMap latent_map, t_map, rope_map, q_map;
+  if (int32_t rc = GetSlabMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, kVSlabs, &latent_map)) return rc;
+  if (int32_t rc = GetSlabMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, 2, &t_map)) return rc;
   if (int32_t rc = GetRowMap(a.pool.rope, a.pool.rope_row_stride, a.pool.pool_rows, kRope, kTile, &rope_map)) return rc;
   if (int32_t rc = GetQMap(a.q, a.q_head_stride, a.q_seq_stride, a.batch, a.heads, kHeads, &q_map)) return rc;
   const int32_t runs = RunsOfDevice();
@@ -1206,7 +1213,7 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   p.merges_by_query = a.batch <= runs ? 1 : 0;
   p.status = status;
   if (int32_t rc = CheckCuda(LaunchOverlapped(MlaDecodeSharedKernel, dim3(2 * static_cast<unsigned>(runs)), dim3(kThreads), kSmemBytes, stream,
-                                              latent_map, rope_map, q_map, p),
+                                              latent_map, t_map, rope_map, q_map, p),
                              "decode_shared launch")) {
     return rc;
   }

@@ -1485,7 +1485,7 @@ namespace {
 int32_t CachedRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, int32_t slabs, CUtensorMap* out) {
   static std::mutex mu;
   static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-  const MapKey key{base, stride, rows, width, slabs > 0 ? -box_rows : box_rows};
+  const MapKey key{base, stride, rows, width, slabs > 0 ? -(box_rows + 1024 * slabs) : box_rows};
   {
     std::lock_guard<std::mutex> lock(mu);
     auto it = cache.find(key);
@@ -1526,10 +1526,10 @@ int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width,
   return CachedRowMap(base, stride, rows, width, box_rows, 0, out);
 }
 
-// The latent columns of a pool as eight slabs of 64; box = 64 rows x four slabs, which land one behind the other, each as a box of
+// The latent columns of a pool as eight slabs of 64; box = 64 rows x some slabs, which land one behind the other, each as a box of
 // GetRowMap would.
-int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, CUtensorMap* out) {
-  return CachedRowMap(base, stride, rows, kLatent, kTile, 4, out);
+int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, int32_t slabs, CUtensorMap* out) {
+  return CachedRowMap(base, stride, rows, kLatent, kTile, slabs, out);
 }
 
 // Query view [batch][heads][576] bf16 with element strides (q_seq_stride, q_head_stride, 1);
