@@ -352,7 +352,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Item mine;
     long long n = 0;
     int n_items = 0;
-#pragma unroll 4
+#pragma unroll 2
     for (int b = stretch; b < stretch_end; ++b) {
       bool second;
       mine = ItemAt(p, b, &second);
@@ -452,9 +452,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0 && rank == 0 && p.merges_by_query == 0) p.merges[run] = make_int4(-1, -1, 0, 0);
   if (any_empty) {  // queries that attend over nothing, alone or with one like them
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      Item it;
       bool second;
-      Item it = ItemAt(p, b, &second);
-      if (second) it = ItemAt(p, b - 1, &second);
+      int at = b;
+#pragma unroll 1
+      do {  // (the second of a pair: the pair's)
+        it = ItemAt(p, at--, &second);
+      } while (second);
       if (it.steps() > 0) continue;
       if (threadIdx.x == 0 && p.merges_by_query != 0) p.merges[b] = make_int4(-1, -1, 0, 0);
       int4* out = reinterpret_cast<int4*>(p.out + static_cast<int64_t>(b) * kHeads * kLatent);
@@ -607,35 +611,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (ok) ok = WarpWait(bar(&misc->t_full[0]), g & 1, misc, p.status, 24);
         if (!ok) break;
         ptx::TcFenceAfterSync();
+        if (ptx::ElectOne()) {
 #pragma unroll
-        for (int k = 8; k < 4 * kTSlabs; ++k) {  // T2 and on, whose Q lies in shared memory
-          const int slab = k >> 2, kk = k & 3;
-          if (ptx::ElectOne()) ptx::MmaF16SS(d, DescAt(q_desc, (slab - 2) * kQSlab + kk * 32), DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, k > 8 ? 1u : 0u);
+          for (int k = 8; k < 4 * kTSlabs; ++k) {  // T2 and on, whose Q lies in shared memory
+            const int slab = k >> 2, kk = k & 3;
+            ptx::MmaF16SS(d, DescAt(q_desc, (slab - 2) * kQSlab + kk * 32), DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, k > 8 ? 1u : 0u);
+          }
+          ptx::TcCommit(bar(&misc->t_empty[0]));
         }
-        if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty[0]));
+        __syncwarp();
         ok = WarpWait(bar(&misc->t_full[1]), g & 1, misc, p.status, 24);
         if (ok && i == 0) ok = WarpWait(bar(&misc->qt_full), seg & 1, misc, p.status, 23);
         if (!ok) break;
         ptx::TcFenceAfterSync();
+        if (ptx::ElectOne()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int slab = k >> 2, kk = k & 3;
-          if (ptx::ElectOne()) ptx::MmaF16TS(d, tmem_u + kColQ + slab * 32 + kk * 8, DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
+          for (int k = 0; k < 8; ++k) {
+            const int slab = k >> 2, kk = k & 3;
+            ptx::MmaF16TS(d, tmem_u + kColQ + slab * 32 + kk * 8, DescAt(t_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
+          }
+          ptx::TcCommit(bar(&misc->t_empty[1]));
         }
-        if (ptx::ElectOne()) ptx::TcCommit(bar(&misc->t_empty[1]));
+        __syncwarp();
         const int set = __shfl_sync(0xffffffffu, g & 1, 0);
         const uint64_t v_desc = DescAt(v_desc0, set * kVSlabs * kSlabBytes);
         ok = WarpWait(bar(&misc->v_full[set]), (g >> 1) & 1, misc, p.status, 26);
         if (!ok) break;
         ptx::TcFenceAfterSync();
+        if (ptx::ElectOne()) {
 #pragma unroll
-        for (int k = 0; k < 4 * kVSlabs; ++k) {
-          const int slab = k >> 2, kk = k & 3;
-          if (ptx::ElectOne()) {
+          for (int k = 0; k < 4 * kVSlabs; ++k) {
+            const int slab = k >> 2, kk = k & 3;
             ptx::MmaF16TS(d, tmem_u + kColQ + (2 + slab) * 32 + kk * 8, DescAt(v_desc, slab * kSlabBytes + kk * 32), kIdesc, 1u);
           }
-        }
-        if (ptx::ElectOne()) {
           ptx::TcCommit(bar(&misc->s_full));
           if (i == n - 1) ptx::TcCommit(bar(&misc->q_empty));
         }
@@ -693,23 +701,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint64_t weights = theirs != 0 ? peer_p_desc : p_desc, values = theirs != 0 ? w_desc : v_desc;
           if (one_pass) {
             const uint32_t keep = theirs != 0 || started != 0 ? 1u : 0u;
+            if (ptx::ElectOne()) {
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k) {
-              if (ptx::ElectOne()) ptx::MmaF16SS(tmem_u + kColO, DescAt(weights, k * 32), DescAt(values, k * 2048), kIdesc, k > 0 ? 1u : keep);
+              for (int k = 0; k < kTile / 16; ++k) {
+                ptx::MmaF16SS(tmem_u + kColO, DescAt(weights, k * 32), DescAt(values, k * 2048), kIdesc, k > 0 ? 1u : keep);
+              }
             }
           } else {
+#pragma unroll 1
             for (int q = 0; q < 2; ++q) {
               if ((active >> q & 1) == 0) continue;
               const uint32_t keep = theirs != 0 ? 1u : (started >> q) & 1;
               const uint32_t off_lo = q == 0 ? 0u : 0xffffffffu;
+              if (ptx::ElectOne()) {
 #pragma unroll
-              for (int k = 0; k < kTile / 16; ++k) {
-                if (ptx::ElectOne()) {
+                for (int k = 0; k < kTile / 16; ++k) {
                   ptx::MmaF16SSLanes(tmem_u + kColO, DescAt(weights, k * 32), DescAt(values, k * 2048), kIdesc, off_lo, ~off_lo, k > 0 ? 1u : keep);
                 }
               }
+              __syncwarp();
             }
           }
+          __syncwarp();
           if (ptx::ElectOne()) {
             if (theirs == 0) {
               ptx::TcCommit(bar(&misc->v_empty[set]));
