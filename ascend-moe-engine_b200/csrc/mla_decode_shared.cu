@@ -41,8 +41,8 @@ namespace b200kv {
 int32_t ValidatePoolView(const b200kv_pool_view* pool);
 int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, CUtensorMap* out);
 int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, int32_t slabs, CUtensorMap* out);
-int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t box_heads,
-                CUtensorMap* out);
+int32_t GetQSlabMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t slabs,
+                    CUtensorMap* out);
 
 namespace {
 
@@ -69,19 +69,20 @@ constexpr int kPBytes = kRows * 128;
 constexpr int kOffPeerP = kOffP + kPBytes;                    // weights of the other CTA's tokens
 constexpr int kOffMisc = kOffPeerP + kPBytes;
 constexpr int kMiscBytes = 4096;
-// An item's slabs of Q for tensor memory come two at a time, through buffers that have no tile then: V's set of the item's first
-// step, T, and V's set again; V's second set, W, and V's second set for a run's first item, whose tiles come at the same time.
+// An item's slabs of Q for tensor memory come two at a time, through buffers that hold nothing then: V's set of the item's first
+// step, T, and V's set again; for a run's first item, whose tiles come at the same time, V's second set, W and both buffers of weights.
 constexpr int kRounds = 3;
-static_assert(2 * kRounds == kQTmemSlabs && 2 * kQSlab <= kVSlabs * kSlabBytes);
+static_assert(2 * kRounds == kQTmemSlabs && 2 * kQSlab <= kVSlabs * kSlabBytes && 2 * kQSlab <= 2 * kPBytes && kOffPeerP == kOffP + kPBytes);
 __device__ __forceinline__ int StageOffset(int round, int seg, int set) {
-  const int v = kOffV + (seg == 0 ? 1 : set) * kVSlabs * kSlabBytes;
-  return round != 1 ? v : seg == 0 ? kOffW : kOffT;
+  if (seg == 0) return round == 0 ? kOffV + kVSlabs * kSlabBytes : round == 1 ? kOffW : kOffP;
+  return round == 1 ? kOffT : kOffV + set * kVSlabs * kSlabBytes;
 }
 constexpr int kSmemBytes = kOffMisc + kMiscBytes + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 
 struct Item {
   int q0, q1;        // q1 < 0: a query alone
+  int row0, row1;    // their table rows
   int len0, len1;
   int lim0, lim1;    // tokens of the common part that each query attends over
   int own;           // where the own tokens begin
@@ -121,9 +122,6 @@ struct Misc {
 static_assert(sizeof(Misc) <= kMiscBytes, "Misc does not fit its reservation");
 
 struct SharedParams {
-  const __nv_bfloat16* q;
-  int64_t q_seq_stride;
-  int64_t q_head_stride;
   const int32_t* block_table;
   int64_t max_blocks;
   int64_t table_rows;
@@ -158,10 +156,12 @@ struct SharedParams {
 // arrays hold, every query belongs to exactly one item.
 __device__ __forceinline__ int StepsOf(int tokens) { return tokens > 0 ? (tokens - 1) / kStep + 1 : 0; }
 
-__device__ __forceinline__ Item MakeItem(int q0, int q1, int len0, int len1, int shared0, int shared1) {
+__device__ __forceinline__ Item MakeItem(int q0, int q1, int row0, int row1, int len0, int len1, int shared0, int shared1) {
   Item it;
   it.q0 = q0;
   it.q1 = q1;
+  it.row0 = row0;
+  it.row1 = row1;
   it.len0 = max(len0, 0);
   it.len1 = q1 >= 0 ? max(len1, 0) : 0;
   it.split = -1;
@@ -193,13 +193,19 @@ __device__ __forceinline__ Item ItemAt(const SharedParams& p, int b, bool* secon
   const int prev = max(b - 1, 0), next = min(b + 1, p.batch - 1);
   const int lead_prev = p.leader[prev], lead = p.leader[b], lead_next = p.leader[next];
   const int len0 = min(p.kv_len[b], p.longest), len1 = min(p.kv_len[next], p.longest), shared0 = p.shared_len[b], shared1 = p.shared_len[next];
+  int row0 = b, row1 = next;
+  if (p.table_index != nullptr) {
+    row0 = p.table_index[b];
+    row1 = p.table_index[next];
+  }
   *second = b > 0 && lead == lead_prev && ((static_cast<unsigned>(prev) - static_cast<unsigned>(lead)) & 1u) == 0;
   const bool pair = next > b && lead == lead_next && ((static_cast<unsigned>(b) - static_cast<unsigned>(lead)) & 1u) == 0;
-  return MakeItem(b, pair ? next : -1, *second ? 0 : len0, pair && !*second ? len1 : 0, shared0, shared1);
+  return MakeItem(b, pair ? next : -1, row0, row1, *second ? 0 : len0, pair && !*second ? len1 : 0, shared0, shared1);
 }
 
 struct Step {
   int query;   // whose table row
+  int row;     // and which
   int token;   // first token
   int valid;   // 1 .. 128 tokens
   int active;  // bit 0: the first query's rows, bit 1: the second's
@@ -210,6 +216,7 @@ __device__ __forceinline__ Step StepAt(const Item& it, int s) {
   if (s < it.common) {
     int tile = s;
     st.query = it.q0;
+    st.row = it.row0;
     if (it.split >= 0 && s > it.split) --tile;
     st.token = tile * kStep;
     const int in0 = it.lim0 - st.token, in1 = it.lim1 - st.token;
@@ -226,6 +233,7 @@ __device__ __forceinline__ Step StepAt(const Item& it, int s) {
   const bool second = s >= it.own0;
   if (second) s -= it.own0;
   st.query = second ? it.q1 : it.q0;
+  st.row = second ? it.row1 : it.row0;
   st.token = it.own + s * kStep;
   st.active = second ? 2 : 1;
   st.valid = min(kStep, (second ? it.len1 : it.len0) - st.token);
@@ -282,7 +290,7 @@ __device__ __forceinline__ bool WarpWait(uint32_t bar, uint32_t parity, Misc* mi
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     MlaDecodeSharedKernel(const __grid_constant__ CUtensorMap latent_map, const __grid_constant__ CUtensorMap t_map,
                           const __grid_constant__ CUtensorMap rope_map, const __grid_constant__ CUtensorMap q_map,
-                          const __grid_constant__ SharedParams p) {
+                          const __grid_constant__ CUtensorMap q_rope_map, const __grid_constant__ SharedParams p) {
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t raw = ptx::SmemAddr(smem_dyn);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -332,6 +340,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::PrefetchTensorMap(&t_map);
     ptx::PrefetchTensorMap(&rope_map);
     ptx::PrefetchTensorMap(&q_map);
+    ptx::PrefetchTensorMap(&q_rope_map);
   }
   if (warp == 5) {
     ptx::TmemAlloc(ptx::SmemAddr(&misc->tmem_base), kTmemCols);
@@ -480,10 +489,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int in_step = tile * kTile;
       if (in_step >= st.valid) return static_cast<int32_t>(p.pool_rows);
       const int token = st.token + in_step;
-      const int64_t table_row = p.table_index != nullptr ? p.table_index[st.query] : st.query;
       const int64_t column = token / p.block_size;
-      const bool inside = table_row >= 0 && table_row < p.table_rows && column < p.max_blocks;
-      const int64_t block = inside ? p.block_table[table_row * p.max_blocks + column] : -1;
+      const bool inside = st.row >= 0 && st.row < p.table_rows && column < p.max_blocks;
+      const int64_t block = inside ? p.block_table[st.row * p.max_blocks + column] : -1;
       const int64_t row = block * p.block_size + token % p.block_size;
       if (block < 0 || row + kTile > p.pool_rows) {
         RecordError(p.status, B200KV_DEV_BAD_BLOCK, st.query, static_cast<int32_t>(column), static_cast<int32_t>(block));
@@ -514,34 +522,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (is_w) {
         if (g > 1) ok = WarpWait(bar(&misc->v_empty[g & 1]), ((g >> 1) & 1) ^ 1, misc, p.status, 12);
         if (!ok) break;
-        // A box is the 64 heads of one query: which of the two is the lane's last bit.
-        const int which = lane & 1, query = which == 0 ? item.q0 : item.q1;
-        const uint32_t slab_bytes = kQSlabBytes * (item.q1 >= 0 ? 2 : 1);
-        auto staged = [&](int round, int of_two) {
-          const int slab = 2 * round + of_two;
+        // A box is 64 heads of both queries (alone, the first brings its neighbour, or zeros, whose rows no one reads).
+        auto staged = [&](int round) {
           const uint32_t full = bar(&misc->stage_full[round]);
-          if (of_two == 0 && which == 0) ptx::MbarArriveExpectTx(full, 2 * slab_bytes);
-          if (query >= 0) {
-            const int x = 64 * (slab < 2 ? kVSlabs * (1 - rank) + slab : kVSlabs * rank + slab - 2);
-            ptx::TmaLoad3D(base + StageOffset(round, seg, g & 1) + of_two * kQSlab + which * kQSlabBytes, &q_map, x, 0, query, full);
-          }
+          ptx::MbarArriveExpectTx(full, 2 * kQSlab);
+          ptx::TmaLoad4D(base + StageOffset(round, seg, g & 1), &q_map, 0, 0, item.q0, round == 0 ? kVSlabs * (1 - rank) : kVSlabs * rank + 2 * round - 2, full);
         };
-        if (lane < 8) staged(lane >> 2, (lane >> 1) & 1);
-        __syncwarp();
-        if (lane < 2 * kQSmemSlabs) {  // the slabs in shared memory: T2, T3, rope
-          const int slab = lane >> 1;
-          const uint32_t full = bar(&misc->q_full);
-          if (lane == 0) ptx::MbarArriveExpectTx(full, kQSmemSlabs * slab_bytes);
-          if (query >= 0) {
-            const int x = slab == 2 ? kLatent : 64 * (kVSlabs * (1 - rank) + 2 + slab);
-            ptx::TmaLoad3D(base + kOffQ + slab * kQSlab + which * kQSlabBytes, &q_map, x, 0, query, full);
-          }
+        if (lane == 0) {
+          staged(0);
+          staged(1);
+          if (seg == 0) staged(2);
+          const uint32_t full = bar(&misc->q_full);  // the slabs in shared memory: T2, T3, rope
+          ptx::MbarArriveExpectTx(full, kQSmemSlabs * kQSlab);
+          ptx::TmaLoad4D(base + kOffQ, &q_map, 0, 0, item.q0, kVSlabs * (1 - rank) + 2, full);
+          ptx::TmaLoad4D(base + kOffQ + 2 * kQSlab, &q_rope_map, 0, 0, item.q0, kLatent / 64, full);
         }
         __syncwarp();
-        ok = WarpWait(bar(&misc->stage_empty[0]), seg & 1, misc, p.status, 13);
-        if (!ok) break;
-        if (lane < 4) staged(2, lane >> 1);
-        __syncwarp();
+        if (seg > 0) {
+          ok = WarpWait(bar(&misc->stage_empty[0]), seg & 1, misc, p.status, 13);
+          if (!ok) break;
+          if (lane == 0) staged(2);
+          __syncwarp();
+        }
       }
       for (int s = lo; s < hi; ++s, ++g) {
         const int32_t row = tile_row(StepAt(item, s), is_w ? 1 - rank : rank);
@@ -555,7 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const bool first_use = g == 0 && !is_w;
         uint32_t parity = every ? (g & 1) ^ 1 : ((g >> 1) & 1) ^ 1;
         if (seg == 0 ? (is_w ? g == 0 : !is_t && g == 1) : s == lo && !is_w) {
-          empty = bar(&misc->stage_empty[every ? 1 : kRounds - 1]);
+          empty = bar(&misc->stage_empty[every ? 1 : seg == 0 ? 0 : 2]);
           parity = seg & 1;
         }
         // The warp polls together; a lane issues its slab the moment its buffer has been given back.
@@ -1191,16 +1193,14 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
     }
     configured_device = device;
   }
-  CUtensorMap latent_map, t_map, rope_map, q_map;
+  CUtensorMap latent_map, t_map, rope_map, q_map, q_rope_map;
   if (int32_t rc = GetSlabMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, kVSlabs, &latent_map)) return rc;
   if (int32_t rc = GetSlabMap(a.pool.latent, a.pool.latent_row_stride, a.pool.pool_rows, 2, &t_map)) return rc;
   if (int32_t rc = GetRowMap(a.pool.rope, a.pool.rope_row_stride, a.pool.pool_rows, kRope, kTile, &rope_map)) return rc;
-  if (int32_t rc = GetQMap(a.q, a.q_head_stride, a.q_seq_stride, a.batch, a.heads, kHeads, &q_map)) return rc;
+  if (int32_t rc = GetQSlabMap(a.q, a.q_head_stride, a.q_seq_stride, a.batch, kHeads, 2, &q_map)) return rc;
+  if (int32_t rc = GetQSlabMap(a.q, a.q_head_stride, a.q_seq_stride, a.batch, kHeads, 1, &q_rope_map)) return rc;
   const int32_t runs = RunsOfDevice();
   SharedParams p{};
-  p.q = static_cast<const __nv_bfloat16*>(a.q);
-  p.q_seq_stride = a.q_seq_stride;
-  p.q_head_stride = a.q_head_stride;
   p.block_table = a.block_table;
   p.max_blocks = a.max_blocks;
   p.table_rows = a.table_rows;
@@ -1226,7 +1226,7 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   p.merges_by_query = a.batch <= runs ? 1 : 0;
   p.status = status;
   if (int32_t rc = CheckCuda(LaunchOverlapped(MlaDecodeSharedKernel, dim3(2 * static_cast<unsigned>(runs)), dim3(kThreads), kSmemBytes, stream,
-                                              latent_map, t_map, rope_map, q_map, p),
+                                              latent_map, t_map, rope_map, q_map, q_rope_map, p),
                              "decode_shared launch")) {
     return rc;
   }

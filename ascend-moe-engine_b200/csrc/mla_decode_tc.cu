@@ -1543,9 +1543,10 @@ struct QKey {
   int32_t batch;
   int32_t heads;
   int32_t box_heads;
+  int32_t slabs;
   bool operator==(const QKey& o) const {
     return base == o.base && head_stride == o.head_stride && seq_stride == o.seq_stride && batch == o.batch && heads == o.heads &&
-           box_heads == o.box_heads;
+           box_heads == o.box_heads && slabs == o.slabs;
   }
 };
 struct QKeyHash {
@@ -1553,19 +1554,19 @@ struct QKeyHash {
     size_t h = reinterpret_cast<size_t>(k.base);
     h ^= static_cast<size_t>(k.head_stride) * 0x9E3779B97F4A7C15ull;
     h ^= static_cast<size_t>(k.seq_stride) * 0xC2B2AE3D27D4EB4Full;
-    return h ^ (static_cast<size_t>(k.batch) * 0x165667B19E3779F9ull) ^ (static_cast<size_t>(k.heads) << 32) ^ (static_cast<size_t>(k.box_heads) << 8);
+    return h ^ (static_cast<size_t>(k.batch) * 0x165667B19E3779F9ull) ^ (static_cast<size_t>(k.heads) << 32) ^ (static_cast<size_t>(k.box_heads) << 8) ^
+           static_cast<size_t>(k.slabs);
   }
 };
 
-}  // namespace
-
-int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t box_heads,
-                CUtensorMap* out) {
+// slabs > 0: the columns as nine slabs of 64 in a dimension of their own; box = 64 columns x heads x two sequences x slabs.
+int32_t CachedQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t box_heads,
+                   int32_t slabs, CUtensorMap* out) {
   static std::mutex mu;
   static std::unordered_map<QKey, CUtensorMap, QKeyHash> cache;
   // A batch of one has no meaningful sequence stride; any multiple of 16 bytes that covers a sequence will do.
   const int64_t seq_stride_eff = batch > 1 ? seq_stride : static_cast<int64_t>(heads) * head_stride;
-  const QKey key{base, head_stride, seq_stride_eff, batch, heads, box_heads};
+  const QKey key{base, head_stride, seq_stride_eff, batch, heads, box_heads, slabs};
   {
     std::lock_guard<std::mutex> lock(mu);
     auto it = cache.find(key);
@@ -1579,12 +1580,13 @@ int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32
     SetLastError("cuTensorMapEncodeTiled could not be resolved from the CUDA driver");
     return B200KV_ERR_RUNTIME;
   }
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kLatent + kRope), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(seq_stride_eff) * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), 1};
-  const cuuint32_t elem[3] = {1, 1, 1};
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(slabs > 0 ? 64 : kLatent + kRope), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch),
+                              (kLatent + kRope) / 64};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(seq_stride_eff) * 2, 128};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_heads), slabs > 0 ? 2u : 1u, static_cast<cuuint32_t>(slabs)};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
   CUtensorMap map;
-  const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+  const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, slabs > 0 ? 4 : 3, const_cast<void*>(base), dims, strides, box,
                              elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) {
@@ -1600,6 +1602,19 @@ int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32
   }
   *out = map;
   return B200KV_OK;
+}
+
+}  // namespace
+
+int32_t GetQMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t box_heads,
+                CUtensorMap* out) {
+  return CachedQMap(base, head_stride, seq_stride, batch, heads, box_heads, 0, out);
+}
+
+// Two sequences' queries, some slabs of 64 columns: a slab of the box is a box of GetQMap for each of the two.
+int32_t GetQSlabMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t slabs,
+                    CUtensorMap* out) {
+  return CachedQMap(base, head_stride, seq_stride, batch, heads, heads, slabs, out);
 }
 
 // Row-major [rows][128] one-byte view (FP8 vectors of 128) with a row stride of `stride_bytes`; box = the whole
