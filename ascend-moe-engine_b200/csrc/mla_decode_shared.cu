@@ -832,8 +832,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const bool whole = lo == 0 && ends;
         const int slot = 2 * run + (lo == 0 ? 1 : 0);
         const int query = which == 0 ? item.q0 : item.q1;
-        const float inv_l = 1.0f / l_all;
         const bool nothing = l_all == 0.0f;  // no weights, and O may hold anything
+        const float inv_l = nothing ? 0.0f : 1.0f / l_all;
         if (rank == 0) {
           if (row == 0 && ends) {
             if (p.merges_by_query != 0) {
@@ -867,6 +867,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 dst[k * kRows] = make_uint4(o[k >> 3][j], o[k >> 3][j + 1], o[k >> 3][j + 2], o[k >> 3][j + 3]);
               }
             } else {
+              if (__any_sync(0xffffffffu, nothing)) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) o[j >> 5][j & 31] = nothing ? 0u : o[j >> 5][j & 31];
+              }
               // A lane has a row; the rows' 128 bytes change places in the warp's part of the weights' buffer, so that a store
               // instruction writes four rows' and not a piece of each of 32.
 #pragma unroll
@@ -875,8 +879,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int j = 8 * (k & 3) + 2 * e;
-                  const __nv_bfloat162 t = __floats2bfloat162_rn(nothing ? 0.0f : __uint_as_float(o[k >> 2][j]) * inv_l,
-                                                                 nothing ? 0.0f : __uint_as_float(o[k >> 2][j + 1]) * inv_l);
+                  const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(o[k >> 2][j]) * inv_l, __uint_as_float(o[k >> 2][j + 1]) * inv_l);
                   two[e] = *reinterpret_cast<const uint32_t*>(&t);
                 }
                 ptx::StShared128(p_row + ((k ^ (row & 7)) << 4), two[0], two[1], two[2], two[3]);
