@@ -73,11 +73,11 @@ namespace {
 
 // From how many common tokens (counted once a pair of neighbours) for each sequence of the step, and from what part of all tokens
 // on, attention goes through the entry point for shared rows. Both sides measured (us a layer, b200kv_mla_decode -> _shared; all
-// sequences share the given length and have 100 tokens of their own): 2 x 512 12.3 -> 12.9, 2 x 2,048 17.2 -> 14.9, 2 x 8,192
-// 22.8 -> 19.0, 4 x 1,024 14.2 -> 15.3, 4 x 4,096 19.6 -> 18.3, 8 x 1,024 17.5 -> 17.4, 8 x 2,048 18.4 -> 19.0, 8 x 8,192 28.5 -> 25.7,
-// 16 x 512 16.0 -> 17.7, 16 x 2,048 21.7 -> 20.9, 16 x 8,192 39.3 -> 31.1, 32 x 512 17.7 -> 20.4, 32 x 2,048 28.4 -> 26.3, 32 x 8,192
-// 61.6 -> 45.7, 32 x 32,768 199 -> 124.
-constexpr int64_t kLeastCommon = 1024;
+// sequences share the given length and have 100 tokens of their own): 2 x 512 12.2 -> 12.4, 2 x 1,024 14.0 -> 12.8, 2 x 8,192
+// 23.0 -> 19.7, 4 x 512 12.6 -> 12.9, 4 x 1,024 14.2 -> 14.6, 4 x 4,096 19.6 -> 17.9, 8 x 512 13.4 -> 14.4, 8 x 1,024 17.5 -> 16.9, 8 x 8,192
+// 28.6 -> 24.9, 16 x 512 15.9 -> 17.3, 16 x 1,024 19.4 -> 18.3, 16 x 8,192 39.6 -> 30.5, 32 x 512 17.7 -> 19.9, 32 x 1,024 22.4 -> 21.7,
+// 32 x 2,048 28.3 -> 25.6, 32 x 8,192 61.8 -> 45.7, 32 x 32,768 199 -> 122.
+constexpr int64_t kLeastCommon = 512;
 constexpr int64_t kCommonPart = 4;
 
 int32_t Refuse(const char* text) {

@@ -16,8 +16,8 @@
 //
 // The two CTAs keep one running maximum: each sends its 128 rows' maxima over its tokens to the other before it exponentiates
 // (one asynchronous 4-byte store a thread), and both come to the same reference. As in the other kernels O is rescaled only when
-// the maximum grows by more than 2^8, so the rounding of P to bf16 (relative 2^-9 of every weight, unbiased; sums and the
-// log-sum-exp take the unrounded fp32 weights) is the only one below fp32.
+// the maximum grows by more than 2^8. The tensor cores take P in bf16, each weight off by at most 2^-8 of itself: the only rounding
+// below fp32 before the result's own (sums and the log-sum-exp take the fp32 weights).
 //
 // The list of work. A pair of queries is an item of n steps: first the tokens that both share (or a prefix of them: the tokens
 // of one sequence each attend up to themselves), then the first query's own tokens, then the second's, all into the same
@@ -26,8 +26,15 @@
 // the second kernel merges. A tile of tokens that is complete for one of the two queries only is two steps, one per query,
 // so that a NaN or an infinity in a row behind a query's end never meets that query's weights (0 x NaN).
 //
-// Warps 0-3: softmax and epilogue (thread = row), 4 and 7: loads, 5: QK, 6: PV. Every wait is bounded; the CTAs of a pair leave
-// together through the cluster barrier.
+// Warps 0-3: softmax and epilogue (thread = row), 4: T and V, 5: QK, 6: PV, 7: Q and W. Every wait is bounded; the CTAs of a pair
+// leave together through the cluster barrier.
+//
+// What bounds it. The matrix instructions of a step take 2,365 cycles (measured alone: 1,354 and 1,032 for S and O; neither tiles
+// arriving at 54 bytes a cycle nor shared-memory stores slow them down). A step takes 3,100 to 3,500: S needs T, whose one buffer is
+// filled anew every step, and the softmax of a step (2,400 cycles with the exchange of maxima) stands between its S and its O. Another
+// item costs 2.5 steps more, a call 4.5 us until S comes for the first time, 2.3 us for partials at the rate at which an SM can
+// write, and 7 us for the merge. 128 sequences behind 8,192 common tokens: 134 us (1,120 TFLOP/s), 157 us when they follow one another
+// for long: the GPU is at its power limit then, with the clock at 1.65 GHz.
 #include <cuda.h>
 
 #include <climits>
@@ -395,7 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const long long cost = Cut::Pos(total, total_items > 0 ? total_items - 1 : 0);
     // No more runs than steps' cost: a run's share is at least a step's, so that none between two of an item's is empty. And no
     // more than pays: r runs take a step's 1.7 us times steps / r, and their parts cost the merge some 0.13 us times r / items
-    // (two queries of 16,384 tokens: 41 runs 23.5 us, all 74 of them 28.4; from 8 queries of 8,192 on it is all of them).
+    // (two queries of 16,384 tokens: 41 runs 23.7 us, all 74 of them 27.5; from 8 queries of 8,192 on it is all of them).
     const long long paying = static_cast<long long>(sqrtf(13.0f * static_cast<float>(total) * static_cast<float>(total_items)));
     const Cut cut{cost, max(1ll, min(static_cast<long long>(runs), min(cost / Cut::kStepCost, paying)))};
     const long long k_lo = run < cut.runs ? cut.First(run) : cost, k_hi = run < cut.runs ? cut.First(run + 1) : cost;
@@ -1034,7 +1041,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Merges what the runs left of every item that was cut. A CTA takes 32 rows x kColumns columns of one. A warp has eight rows x four
 // quads of columns: it reads 128 bytes of a quad's rows and writes 32 bytes of a row, and goes over the strips of 16 columns of its
 // half of the CTA's columns; with 16 columns a CTA the two halves of the warps share the parts out instead (an item of few queries
-// and many parts: 66 parts of one took 17 us with 32 columns a CTA). The rows' weights are worked out once, by the whole CTA.
+// and many parts: two queries of 16,384 tokens 27.9 us a call with 32 columns a CTA, 23.8 with 16). The rows' weights are worked out once, by the whole CTA.
 constexpr int kMergeParts = 128;  // more than runs there are
 constexpr int kMergeRows = 32;
 
@@ -1233,16 +1240,16 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
                              "decode_shared launch")) {
     return rc;
   }
-  // The fewer queries, the fewer items there can be to merge, and the more parts they have: fewer columns a CTA, so that half the
-  // queries' items give some four CTAs an SM (32 x 4,096 tokens: 41.9 us a call with 128 columns, 39.6 with 32; 497 queries of up to
-  // 200 tokens: 56.1 with 256 columns, 52.1 with 128; 80 queries of some 3,000: 65.7 with 256, 63.2 with 128, 64.9 with 32).
+  // The fewer queries, the fewer items there can be to merge, and the more parts they have: fewer columns a CTA, so that there are
+  // enough CTAs. Sequences behind a common prefix, us a call with 16, 32, 64 and 128 columns: 4 x 8,192 21.4, 23.8, 27.2, 35.3;
+  // 8 x 8,192 23.9, 24.8, 27.3, 33.4; 16 x 4,096 24.8, 23.3, 24.6, 28.1; 32 x 4,096 36.5, 33.0, 32.8, 33.1; 48 x 4,096 47.5, 41.6, 40.5,
+  // 39.7; 256 x 1,024 73.0, 62.0, 59.3, 57.3.
   const unsigned merges = static_cast<unsigned>(a.batch < runs ? a.batch : runs);
   auto merge = [&](auto kernel, int columns) {
     return LaunchOverlapped(kernel, dim3(static_cast<unsigned>(kRows / kMergeRows * (kLatent / columns)), merges), dim3(256), 0, stream, p);
   };
-  return CheckCuda(a.batch < 5    ? merge(MlaSharedMergeKernel<16>, 16)
-                   : a.batch < 37 ? merge(MlaSharedMergeKernel<32>, 32)
-                   : a.batch < 74 ? merge(MlaSharedMergeKernel<64>, 64)
+  return CheckCuda(a.batch < 12   ? merge(MlaSharedMergeKernel<16>, 16)
+                   : a.batch < 36 ? merge(MlaSharedMergeKernel<32>, 32)
                                   : merge(MlaSharedMergeKernel<128>, 128),
                    "decode_shared merge launch");
 }
