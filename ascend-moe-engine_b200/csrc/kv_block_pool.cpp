@@ -135,6 +135,18 @@ int32_t RowsIn(const b200kv_block_pool* pool, int32_t seq, int32_t index) {  // 
   return static_cast<int32_t>(left < pool->block_size ? left : pool->block_size);
 }
 
+// scratch[block]: the rows that mean something, those of the sequence with the most tokens there.
+void MarkRows(const b200kv_block_pool* pool) {
+  std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
+  for (int32_t s = 0; s < pool->max_seqs; ++s) {
+    const int32_t* row = pool->table + static_cast<size_t>(s) * pool->max_blocks_per_seq;
+    for (int32_t i = 0; i < pool->used_blocks[s]; ++i) {
+      const int32_t rows = RowsIn(pool, s, i);
+      if (rows > pool->scratch[row[i]]) pool->scratch[row[i]] = rows;
+    }
+  }
+}
+
 void NoMove(int32_t* move) {
   move[0] = move[1] = -1;
   move[2] = 0;
@@ -296,8 +308,17 @@ extern "C" int32_t b200kv_block_pool_unshare(b200kv_block_pool* pool, int32_t se
   return B200KV_OK;
 }
 
-// Undoes the unshare that has just been made, when its copy could not be (not part of the C ABI).
+// Not part of the C ABI: for the engine.
 namespace b200kv {
+// Tokens that the blocks hold, those of several sequences once.
+int64_t StoredTokens(const b200kv_block_pool* pool) {
+  MarkRows(pool);
+  int64_t tokens = 0;
+  for (int32_t id = 0; id < pool->num_blocks; ++id) tokens += pool->scratch[id];
+  return tokens;
+}
+
+// Undoes the unshare that has just been made, when its copy could not be.
 void UndoUnshare(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move) {
   if (move[0] < 0) return;
   Drop(pool, move[1], true);
@@ -316,15 +337,7 @@ extern "C" int32_t b200kv_block_pool_plan_compact(b200kv_block_pool* pool, int32
     SetLastError("plan_compact: %d moves into %p", max_moves, static_cast<void*>(moves_out));
     return moves_out == nullptr ? -B200KV_ERR_NULLPTR : -B200KV_ERR_INVALID;
   }
-  // The rows that mean something: what the sequence with the most tokens in a block has there.
-  std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
-  for (int32_t s = 0; s < pool->max_seqs; ++s) {
-    const int32_t* row = pool->table + static_cast<size_t>(s) * pool->max_blocks_per_seq;
-    for (int32_t i = 0; i < pool->used_blocks[s]; ++i) {
-      const int32_t rows = RowsIn(pool, s, i);
-      if (rows > pool->scratch[row[i]]) pool->scratch[row[i]] = rows;
-    }
-  }
+  MarkRows(pool);
   int32_t n = 0, to = 0;
   for (int32_t from = pool->num_blocks - 1; n < max_moves; --from) {
     while (from > to && pool->refs[from] == 0) --from;

@@ -30,6 +30,7 @@ namespace b200kv {
 void SetLastError(const char* fmt, ...);
 int32_t CheckCuda(cudaError_t err, const char* what);
 int32_t FaultCheck(const char* entry_point);
+int64_t StoredTokens(const b200kv_block_pool* pool);
 void UndoUnshare(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move);
 }  // namespace b200kv
 
@@ -62,7 +63,6 @@ struct b200kv_engine {
   int32_t step_tokens = 0;
   int32_t allocations_at_begin = 0;
   int64_t steps = 0;
-  int64_t active_tokens = 0;
   std::vector<int32_t> step_seq_ids;   // sized at Build: the step's sequences and by how much each grew
   std::vector<int32_t> step_grown;
   bool step_shares = false;            // the step's attention is b200kv_mla_decode_shared
@@ -249,10 +249,7 @@ extern "C" int32_t b200kv_engine_admit(b200kv_engine* e, int32_t seq) {
 extern "C" int32_t b200kv_engine_release(b200kv_engine* e, int32_t seq) {
   if (e == nullptr) return B200KV_ERR_NULLPTR;
   if (e->in_step) return Refuse("engine_release: a step is in flight");
-  const int32_t len = b200kv_block_pool_seq_len(e->pool, seq);
-  const int32_t rc = b200kv_block_pool_release(e->pool, seq);
-  if (rc == B200KV_OK && len > 0) e->active_tokens -= len;
-  return rc;
+  return b200kv_block_pool_release(e->pool, seq);
 }
 
 extern "C" int32_t b200kv_engine_begin_step(b200kv_engine* e, const int32_t* seqs, const int32_t* new_tokens,
@@ -338,7 +335,6 @@ extern "C" int32_t b200kv_engine_begin_step(b200kv_engine* e, const int32_t* seq
     return rc;
   }
   e->in_step = true;
-  e->active_tokens += at;
   return B200KV_OK;
 }
 
@@ -352,7 +348,6 @@ extern "C" int32_t b200kv_engine_abort_step(b200kv_engine* e) {
       return rc;
     }
   }
-  e->active_tokens -= e->step_tokens;
   e->in_step = false;
   return b200kv_block_pool_validate(e->pool);
 }
@@ -456,7 +451,6 @@ extern "C" int32_t b200kv_engine_fork(b200kv_engine* e, int32_t src, int32_t dst
       return rc;
     }
   }
-  e->active_tokens += b200kv_block_pool_seq_len(e->pool, dst);
   return B200KV_OK;
 }
 
@@ -481,9 +475,7 @@ extern "C" int32_t b200kv_engine_trim(b200kv_engine* e, int32_t seq, int32_t n_t
       }
     }
   }
-  if (int32_t rc = b200kv_block_pool_ungrow(e->pool, seq, n_tokens)) return rc;
-  e->active_tokens -= n_tokens;
-  return B200KV_OK;
+  return b200kv_block_pool_ungrow(e->pool, seq, n_tokens);
 }
 
 extern "C" int32_t b200kv_engine_compact(b200kv_engine* e, int32_t max_moves, void* stream) {
@@ -512,6 +504,6 @@ extern "C" int32_t b200kv_engine_end_step(b200kv_engine* e) {
 
 extern "C" int64_t b200kv_engine_stats_json(const b200kv_engine* e, char* buffer, int64_t capacity) {
   if (e == nullptr) return -1;
-  return b200kv_paged_attention_stats_json(e->cfg.num_blocks, e->cfg.layers, e->active_tokens, e->cfg.block_size, buffer,
-                                           capacity);
+  return b200kv_paged_attention_stats_json(e->cfg.num_blocks, e->cfg.layers, b200kv::StoredTokens(e->pool), e->cfg.block_size,
+                                           buffer, capacity);
 }

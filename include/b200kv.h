@@ -658,7 +658,8 @@ int32_t b200kv_engine_compact(b200kv_engine* engine, int32_t max_moves, void* st
 /* Abandons the step in flight (a launch of it failed): every sequence gives back what the step added, tables,
  * lengths and the free list are as before begin_step. */
 int32_t b200kv_engine_abort_step(b200kv_engine* engine);
-/* The "paged_attention" object of the reference's diagnostics for the engine's current state. */
+/* The "paged_attention" object of the reference's diagnostics for the engine's current state. A token that several sequences share
+ * counts once. */
 int64_t b200kv_engine_stats_json(const b200kv_engine* engine, char* buffer, int64_t capacity);
 
 /* ------------------------------------------------------------------------------------------------

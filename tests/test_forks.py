@@ -173,6 +173,25 @@ def test_engine_forks_trims_and_compacts_over_host_memory():
     e.abort_step()
 
 
+def test_shared_tokens_count_once_in_the_statistics():
+    e = engine(max_step_tokens=300)
+    tokens = lambda: int(e.stats_json().split('"active_context_tokens": ')[1].split(",")[0])  # noqa: E731
+    e.admit(0)
+    e.begin_step([0], [130])
+    e.end_step()
+    assert tokens() == 130
+    e.fork(0, 1)          # 128 are common, the two behind them copied
+    assert tokens() == 132
+    e.begin_step([1, 0], [3, 1])
+    assert tokens() == 136
+    e.abort_step()
+    assert tokens() == 132
+    e.release(0)
+    assert tokens() == 130
+    e.trim(1, 30)
+    assert tokens() == 100
+
+
 def test_a_copy_that_fails_changes_nothing():
     e = engine(max_step_tokens=300)
     e.admit(0)
