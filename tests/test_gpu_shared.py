@@ -149,6 +149,22 @@ def test_strided_queries():
     Call(case, q=wide[:, :HEADS, :576]).run().check()
 
 
+def test_queries_laid_out_by_head_and_one_query_for_all():
+    case = Case([(128, [130, 200, 128])])
+    Call(case, q=case.q.cuda().transpose(0, 1).contiguous().transpose(0, 1)).run().check()
+    case.q[:] = case.q[0].clone()
+    Call(case, q=case.q[0].cuda()[None].expand(3, -1, -1)).run().check()
+
+
+def test_rows_that_lie_beyond_32_bits():
+    case = Case([(256, [257, 400, 256])]).poison_unused()
+    call, before = Call(case), 2 ** 32 // 1152 // case.block + 1
+    pool = torch.empty(before * case.block + len(case.pool), 576, dtype=torch.bfloat16, device="cuda")
+    pool[before * case.block:] = call.cache[0]
+    call.cache, call.view, call.table = (pool,), b200kv.pool_view(pool), call.table + before
+    call.run().check()
+
+
 def test_quantised_output_is_the_quantisers():
     call = Call(Case([(256, [300, 257, 256])]), quantised=True).run()
     call.check()
