@@ -825,11 +825,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       Item next_item;
       int next_lo, next_hi;
       const bool more = walk.Next(&next_item, &next_lo, &next_hi);
+      if (have) send(l_run);  // (the sum of this item's weights, received in its epilogue)
       if (more) load_q(g & 1);
       if (!have) ptx::ClusterWait();  // (the peer's barriers are touched from here on)
       if (have) {
         // ---- epilogue of the item ----
-        send(l_run);
         const float l_all = l_run + receive();
         ok = WarpWait(bar(&misc->w_empty), (g & 1) ^ 1, misc, p.status, 32) && ok;
         weights_free();
