@@ -5,9 +5,9 @@
 // steps).
 //
 //   Build      reserve the KV spans and the step's staging in the static arena, note the attention workspace,
-//              ONE commit, the workspace, seal; create the block pool; one pinned staging block for the uploads.
+//              ONE commit, the workspace, seal; create the block pool; two pinned staging blocks for the uploads.
 //   step       begin: grow every sequence of the step in the block pool (plan, then commit: a refused growth
-//              changes nothing), write the step's table rows, lengths and slots into the pinned block and upload
+//              changes nothing), write the step's table rows, lengths and slots into a pinned block and upload
 //              them with ONE copy (the reference's mailbox, :515-519). Then per layer, in the reference's stage
 //              order: producer (kv_a_norm + rope + kv_cache_write, stages 6-8), attention (9), MX quantisation of
 //              its output (10). end: no allocation happened since begin, as the reference asserts per step
@@ -52,9 +52,18 @@ struct b200kv_engine {
   int32_t* d_status = nullptr;
   int32_t* d_queries = nullptr;  // [4][max_step_tokens]: kv_len, leader, shared_len, table_index of the step's queries
   int32_t* d_moves = nullptr;    // [num_blocks][3]
-  // One pinned block that mirrors [queries | table .. lens] of the arena byte for byte: one copy uploads a step (from the
-  // table on, when the step's attention needs no queries).
-  unsigned char* staging = nullptr;
+  // Pinned blocks that mirror [queries | table .. lens] of the arena byte for byte: one copy uploads a step (from the
+  // table on, when the step's attention needs no queries). The copy reads its block when the stream comes to it, behind the
+  // kernels of the steps before, so steps take the blocks in turn and one is written again only when its upload has been made.
+  struct Staging {
+    unsigned char* at = nullptr;
+    cudaEvent_t uploaded = nullptr;
+    bool pending = false;
+  };
+  static constexpr int kStagings = 2;
+  Staging stagings[kStagings];
+  int at_staging = 0;
+  unsigned char* staging = nullptr;  // of the step in hand
   size_t staging_bytes = 0;
   size_t table_off = 0, slots_off = 0, lens_off = 0;
   // The step in flight.
@@ -115,6 +124,43 @@ bool PlanQueries(b200kv_engine* e, int32_t n_seqs, int32_t n_tokens) {
   }
   const int64_t common = b200kv_find_shared(table, e->cfg.max_blocks_per_seq, lens, n_seqs, e->cfg.block_size, leader, shared);
   return common >= kLeastCommon * n_seqs && kCommonPart * common >= all;
+}
+
+// The next staging block, once the upload that was last made from it has left it.
+int32_t TakeStaging(b200kv_engine* e) {
+  b200kv_engine::Staging& block = e->stagings[e->at_staging];
+  if (block.pending) {
+    // (a capture on this thread does not mind: the event is none of its)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const int32_t rc = CheckCuda(cudaEventSynchronize(block.uploaded), "engine staging (the upload before)");
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (rc != B200KV_OK) return rc;
+    block.pending = false;
+  }
+  e->staging = block.at;
+  return B200KV_OK;
+}
+
+// The block in hand goes to the device, from byte `from` on. An upload that becomes part of a graph is read when the graph runs and
+// leaves no event.
+int32_t Upload(b200kv_engine* e, size_t from, cudaStream_t stream) {
+  unsigned char* to = reinterpret_cast<unsigned char*>(e->d_queries) + from;
+  if (int32_t rc = b200kv::FaultCheck("b200kv_engine_step_upload")) return rc;
+  if (e->cfg.backend != B200KV_ARENA_DEVICE) {
+    std::memcpy(to, e->staging + from, e->staging_bytes - from);
+  } else {
+    b200kv_engine::Staging& block = e->stagings[e->at_staging];
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (int32_t rc = CheckCuda(cudaStreamIsCapturing(stream, &capture), "engine step upload")) return rc;
+    if (int32_t rc = CheckCuda(cudaMemcpyAsync(to, e->staging + from, e->staging_bytes - from, cudaMemcpyHostToDevice, stream), "engine step upload")) return rc;
+    if (capture == cudaStreamCaptureStatusNone) {
+      if (int32_t rc = CheckCuda(cudaEventRecord(block.uploaded, stream), "engine step upload")) return rc;
+      block.pending = true;
+    }
+  }
+  e->at_staging = (e->at_staging + 1) % b200kv_engine::kStagings;
+  return B200KV_OK;
 }
 
 // Moves of blocks (pool ids) in every layer, enqueued on the stream.
@@ -207,15 +253,18 @@ extern "C" b200kv_engine* b200kv_engine_create(const b200kv_engine_config* confi
   e->slots_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.slot_mapping_handle) - first);
   e->lens_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.seq_lens_handle) - first);
   e->staging_bytes = e->lens_off + static_cast<size_t>(c.max_seqs) * 4;
-  if (c.backend == B200KV_ARENA_DEVICE) {
-    void* pinned = nullptr;
-    if (CheckCuda(cudaMallocHost(&pinned, e->staging_bytes), "engine staging (pinned)") != B200KV_OK) return fail();
-    e->staging = static_cast<unsigned char*>(pinned);
-  } else {
-    e->staging = new (std::nothrow) unsigned char[e->staging_bytes];
-    if (e->staging == nullptr) return fail();
+  for (b200kv_engine::Staging& block : e->stagings) {
+    if (c.backend == B200KV_ARENA_DEVICE) {
+      void* pinned = nullptr;
+      if (CheckCuda(cudaMallocHost(&pinned, e->staging_bytes), "engine staging (pinned)") != B200KV_OK) return fail();
+      block.at = static_cast<unsigned char*>(pinned);
+      if (CheckCuda(cudaEventCreateWithFlags(&block.uploaded, cudaEventDisableTiming), "engine staging (event)") != B200KV_OK) return fail();
+    } else {
+      block.at = new (std::nothrow) unsigned char[e->staging_bytes];
+      if (block.at == nullptr) return fail();
+    }
+    std::memset(block.at, 0, e->staging_bytes);
   }
-  std::memset(e->staging, 0, e->staging_bytes);
   e->pool = b200kv_block_pool_create(c.num_blocks, c.block_size, c.max_seqs, c.max_blocks_per_seq, nullptr);
   if (e->pool == nullptr) return fail();
   e->step_seq_ids.resize(static_cast<size_t>(c.max_seqs));
@@ -228,8 +277,10 @@ extern "C" b200kv_engine* b200kv_engine_create(const b200kv_engine_config* confi
 extern "C" void b200kv_engine_destroy(b200kv_engine* e) {
   if (e == nullptr) return;
   if (e->pool != nullptr) b200kv_block_pool_destroy(e->pool);
-  if (e->staging != nullptr) {
-    if (e->cfg.backend == B200KV_ARENA_DEVICE) cudaFreeHost(e->staging); else delete[] e->staging;
+  for (b200kv_engine::Staging& block : e->stagings) {
+    if (block.uploaded != nullptr) cudaEventDestroy(block.uploaded);
+    if (block.at == nullptr) continue;
+    if (e->cfg.backend == B200KV_ARENA_DEVICE) cudaFreeHost(block.at); else delete[] block.at;
   }
   if (e->arena != nullptr) b200kv_arena_destroy(e->arena);
   delete e;
@@ -294,6 +345,7 @@ extern "C" int32_t b200kv_engine_begin_step(b200kv_engine* e, const int32_t* seq
                  b200kv_block_pool_free_count(e->pool));
     return B200KV_ERR_INVALID;
   }
+  if (int32_t rc = TakeStaging(e)) return rc;
   // COMMIT: grow, and mirror the step into the pinned block: table rows in step order, lengths, slots.
   int32_t* s_table = reinterpret_cast<int32_t*>(e->staging + e->table_off);
   int32_t* s_slots = reinterpret_cast<int32_t*>(e->staging + e->slots_off);
@@ -318,18 +370,7 @@ extern "C" int32_t b200kv_engine_begin_step(b200kv_engine* e, const int32_t* seq
   e->step_tokens = at;
   // ONE upload per step: the queries, the table rows, the slots and the lengths lie in the arena in this order. An upload
   // that fails takes the step's growth back: the call changed nothing.
-  const size_t from = e->step_shares ? 0 : e->table_off;
-  unsigned char* to = reinterpret_cast<unsigned char*>(e->d_queries) + from;
-  int32_t rc = b200kv::FaultCheck("b200kv_engine_step_upload");
-  if (rc == B200KV_OK) {
-    if (e->cfg.backend == B200KV_ARENA_DEVICE) {
-      rc = CheckCuda(cudaMemcpyAsync(to, e->staging + from, e->staging_bytes - from, cudaMemcpyHostToDevice,
-                                     static_cast<cudaStream_t>(stream)),
-                     "engine step upload");
-    } else {
-      std::memcpy(to, e->staging + from, e->staging_bytes - from);
-    }
-  }
+  const int32_t rc = Upload(e, e->step_shares ? 0 : e->table_off, static_cast<cudaStream_t>(stream));
   if (rc != B200KV_OK) {
     for (int32_t i = n_seqs - 1; i >= 0; --i) b200kv_block_pool_ungrow(e->pool, seqs[i], e->step_grown[static_cast<size_t>(i)]);
     return rc;
