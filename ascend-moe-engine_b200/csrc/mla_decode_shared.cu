@@ -41,6 +41,7 @@
 
 #include "common.cuh"
 #include "mla_tc_common.cuh"
+#include "shared_merge_record.h"
 #include "sm100_ptx.cuh"
 
 namespace b200kv {
@@ -151,12 +152,15 @@ struct SharedParams {
   float* ws_m;  // [slot][128], log2 domain
   float* ws_l;
   Item* items;   // [batch]: the items, in order (those of a run are written by the run's CTAs)
-  // What there is to merge: an item's queries, the run that began it, the run that finished it; x < 0: nothing. By the item's
-  // first query where the batch has no more queries than there are runs, else by the run that finished it.
-  int4* merges;
+  // What there is to merge. By the item's first query where the batch has no more queries than there are runs, else by the run that
+  // finished it.
+  MergeRecord* merges;
   int32_t merges_by_query;
+  int32_t runs;
   int32_t* status;
 };
+
+__device__ __forceinline__ MergeRecord NothingToMerge() { return {-1, -1, 0, 0}; }
 
 // ---- the list of work -------------------------------------------------------------------------------------------------
 // Query b is the second of a pair if the one before it has the same leader and stands at an even distance from it. Whatever the
@@ -465,7 +469,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::TcFenceBeforeSync();
   any_empty = __syncthreads_or(any_empty) != 0;
   ptx::TcFenceAfterSync();
-  if (threadIdx.x == 0 && rank == 0 && p.merges_by_query == 0) p.merges[run] = make_int4(-1, -1, 0, 0);
+  if (threadIdx.x == 0 && rank == 0 && p.merges_by_query == 0) p.merges[run] = NothingToMerge();
   if (any_empty) {  // queries that attend over nothing, alone or with one like them
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
       Item it;
@@ -476,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         it = ItemAt(p, at--, &second);
       } while (second);
       if (it.steps() > 0) continue;
-      if (threadIdx.x == 0 && p.merges_by_query != 0) p.merges[b] = make_int4(-1, -1, 0, 0);
+      if (threadIdx.x == 0 && p.merges_by_query != 0) p.merges[b] = NothingToMerge();
       int4* out = reinterpret_cast<int4*>(p.out + static_cast<int64_t>(b) * kHeads * kLatent);
       for (int i = threadIdx.x; i < kHeads * kLatent / 8; i += kThreads) out[i] = make_int4(0, 0, 0, 0);
       if (p.lse != nullptr && threadIdx.x < kHeads) p.lse[static_cast<int64_t>(b) * kHeads + threadIdx.x] = -INFINITY;
@@ -844,10 +848,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (rank == 0) {
           if (row == 0 && ends) {
             if (p.merges_by_query != 0) {
-              p.merges[item.q0] = continued ? make_int4(item.q0, item.q1, misc->began_in, run) : make_int4(-1, -1, 0, 0);
-              if (item.q1 >= 0) p.merges[item.q1] = make_int4(-1, -1, 0, 0);
+              p.merges[item.q0] = continued ? MergeRecord{item.q0, item.q1, misc->began_in, run} : NothingToMerge();
+              if (item.q1 >= 0) p.merges[item.q1] = NothingToMerge();
             } else if (continued) {
-              p.merges[run] = make_int4(item.q0, item.q1, misc->began_in, run);
+              p.merges[run] = MergeRecord{item.q0, item.q1, misc->began_in, run};
             }
           }
           if (!whole) {
@@ -1042,7 +1046,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // quads of columns: it reads 128 bytes of a quad's rows and writes 32 bytes of a row, and goes over the strips of 16 columns of its
 // half of the CTA's columns; with 16 columns a CTA the two halves of the warps share the parts out instead (an item of few queries
 // and many parts: two queries of 16,384 tokens 27.9 us a call with 32 columns a CTA, 23.8 with 16). The rows' weights are worked out once, by the whole CTA.
-constexpr int kMergeParts = 128;  // more than runs there are
 constexpr int kMergeRows = 32;
 
 // kStrips strips of kParts parts are in flight at a time: eight loads a thread, whatever the number of parts. The first eight are
@@ -1111,10 +1114,11 @@ __global__ void __launch_bounds__(256) MlaSharedMergeKernel(const __grid_constan
   __shared__ float4 s_other[kColumns == 16 ? 128 : 1];
   GridDependencyWait();
   GridDependencyTrigger();
-  const int4 merge = p.merges[blockIdx.y];
-  const int query = rows < kHeads ? merge.x : merge.y;
-  if (merge.x < 0 || query < 0) return;
-  const int first = merge.z, parts = merge.w - first + 1;
+  const MergeRecord merge = p.merges[blockIdx.y];
+  if (!MergeHolds(merge, static_cast<int>(blockIdx.y), p.merges_by_query != 0, p.batch, p.runs)) return;
+  const int query = rows < kHeads ? merge.q0 : merge.q1;
+  if (query < 0) return;
+  const int first = merge.first, parts = merge.last - first + 1;
   constexpr bool kSplit = kColumns == 16;
   constexpr int kStrips = kSplit ? 1 : kColumns / 32;
   const int mine = 8 * (warp & 3) + (lane & 7);                                                 // this thread's row of the 32
@@ -1184,7 +1188,7 @@ int32_t RunsOfDevice() { return CurrentDeviceSmCount() / 2 < kMergeParts ? Curre
 
 size_t SharedWorkspaceBytes(int32_t batch) {
   const size_t slots = static_cast<size_t>(RunsOfDevice()) * 2;
-  return slots * kRows * (kLatent + 2) * sizeof(float) + static_cast<size_t>(RunsOfDevice()) * sizeof(int4) + static_cast<size_t>(batch) * sizeof(Item);
+  return slots * kRows * (kLatent + 2) * sizeof(float) + static_cast<size_t>(RunsOfDevice()) * sizeof(MergeRecord) + static_cast<size_t>(batch) * sizeof(Item);
 }
 
 bool SharedSupports(const b200kv_shared_args& a) {
@@ -1231,9 +1235,10 @@ int32_t LaunchShared(const b200kv_shared_args& a, cudaStream_t stream, int32_t* 
   p.ws_o = static_cast<float4*>(a.workspace);
   p.ws_m = reinterpret_cast<float*>(p.ws_o + slots * kRows * (kLatent / 4));
   p.ws_l = p.ws_m + slots * kRows;
-  p.merges = reinterpret_cast<int4*>(p.ws_l + slots * kRows);
+  p.merges = reinterpret_cast<MergeRecord*>(p.ws_l + slots * kRows);
   p.items = reinterpret_cast<Item*>(p.merges + runs);
   p.merges_by_query = a.batch <= runs ? 1 : 0;
+  p.runs = runs;
   p.status = status;
   if (int32_t rc = CheckCuda(LaunchOverlapped(MlaDecodeSharedKernel, dim3(2 * static_cast<unsigned>(runs)), dim3(kThreads), kSmemBytes, stream,
                                               latent_map, t_map, rope_map, q_map, q_rope_map, p),
