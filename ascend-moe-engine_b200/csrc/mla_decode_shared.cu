@@ -47,6 +47,9 @@
 namespace b200kv {
 
 int32_t ValidatePoolView(const b200kv_pool_view* pool);
+int32_t SimtSplitCount(int32_t batch, int32_t sms);
+size_t SimtWorkspaceBytes(int32_t batch, int32_t heads, int32_t sms);
+size_t TcWorkspaceBytes(int32_t n_ctas);
 int32_t GetRowMap(const void* base, int64_t stride, int64_t rows, int32_t width, int32_t box_rows, CUtensorMap* out);
 int32_t GetSlabMap(const void* base, int64_t stride, int64_t rows, int32_t slabs, CUtensorMap* out);
 int32_t GetQSlabMap(const void* base, int64_t head_stride, int64_t seq_stride, int32_t batch, int32_t heads, int32_t slabs,
@@ -1266,8 +1269,12 @@ using namespace b200kv;
 
 extern "C" size_t b200kv_mla_decode_shared_workspace_bytes(int32_t batch, int32_t heads) {
   if (batch <= 0 || heads <= 0) return 0;
-  const size_t own = SharedWorkspaceBytes(batch), plain = b200kv_mla_decode_workspace_bytes(batch, heads, 0);
-  return own > plain ? own : plain;
+  // Beside the kernel's own need that of b200kv_mla_decode, where another geometry goes: its CUDA-core form keeps partials only
+  // where it splits sequences, which many queries are not.
+  const int32_t sms = CurrentDeviceSmCount();
+  size_t need = SharedWorkspaceBytes(batch);
+  for (size_t other : {TcWorkspaceBytes(sms), SimtSplitCount(batch, sms) > 1 ? SimtWorkspaceBytes(batch, heads, sms) : 0}) need = other > need ? other : need;
+  return need;
 }
 
 extern "C" int32_t b200kv_mla_decode_shared(const b200kv_shared_args* args, void* stream, b200kv_status_word* status) {
