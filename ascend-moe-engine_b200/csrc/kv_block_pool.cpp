@@ -318,6 +318,31 @@ int64_t StoredTokens(const b200kv_block_pool* pool) {
   return tokens;
 }
 
+// Unshare without a free block, for a sequence that is about to lose its tokens behind block `index`: the last block there that only
+// this sequence holds changes places with the common one, which the ungrow that follows lets go of. False: there is none.
+bool TakeFromBehind(b200kv_block_pool* pool, int32_t seq, int32_t index, int32_t* move_out) {
+  int32_t* row = pool->table + static_cast<size_t>(seq) * pool->max_blocks_per_seq;
+  for (int32_t i = pool->used_blocks[seq] - 1; i > index; --i) {
+    if (pool->refs[row[i]] != 1) continue;
+    move_out[0] = row[index];
+    move_out[1] = row[i];
+    move_out[2] = RowsIn(pool, seq, index);
+    row[index] = move_out[1];
+    row[i] = move_out[0];
+    return true;
+  }
+  return false;
+}
+
+// Undoes it when its copy could not be made.
+void UndoTakeFromBehind(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move) {
+  int32_t* row = pool->table + static_cast<size_t>(seq) * pool->max_blocks_per_seq;
+  for (int32_t i = index + 1; i < pool->used_blocks[seq]; ++i) {
+    if (row[i] == move[0]) row[i] = move[1];
+  }
+  row[index] = move[0];
+}
+
 // Undoes the unshare that has just been made, when its copy could not be.
 void UndoUnshare(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move) {
   if (move[0] < 0) return;

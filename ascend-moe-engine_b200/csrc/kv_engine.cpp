@@ -32,6 +32,8 @@ int32_t CheckCuda(cudaError_t err, const char* what);
 int32_t FaultCheck(const char* entry_point);
 int64_t StoredTokens(const b200kv_block_pool* pool);
 void UndoUnshare(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move);
+bool TakeFromBehind(b200kv_block_pool* pool, int32_t seq, int32_t index, int32_t* move_out);
+void UndoTakeFromBehind(b200kv_block_pool* pool, int32_t seq, int32_t index, const int32_t* move);
 }  // namespace b200kv
 
 using b200kv::CheckCuda;
@@ -506,12 +508,18 @@ extern "C" int32_t b200kv_engine_trim(b200kv_engine* e, int32_t seq, int32_t n_t
   const int32_t left = len - n_tokens;
   if (n_tokens > 0 && left % e->cfg.block_size != 0) {  // the block that will be half filled is the sequence's own from here on
     const int32_t index = left / e->cfg.block_size;
+    const int32_t block = b200kv_block_pool_table(e->pool)[static_cast<size_t>(seq) * e->cfg.max_blocks_per_seq + index];
     int32_t move[3];
-    if (int32_t rc = b200kv_block_pool_unshare(e->pool, seq, index, move)) return rc;
+    // (in a full pool the copy goes into a block that this call empties)
+    const bool from_behind = b200kv_block_pool_ref_count(e->pool, block) > 1 && b200kv_block_pool_free_count(e->pool) == 0 &&
+                             b200kv::TakeFromBehind(e->pool, seq, index, move);
+    if (!from_behind) {
+      if (int32_t rc = b200kv_block_pool_unshare(e->pool, seq, index, move)) return rc;
+    }
     if (move[0] >= 0) {
       if (move[2] > left % e->cfg.block_size) move[2] = left % e->cfg.block_size;
       if (int32_t rc = CopyMoves(e, move, 1, stream)) {
-        b200kv::UndoUnshare(e->pool, seq, index, move);
+        (from_behind ? b200kv::UndoTakeFromBehind : b200kv::UndoUnshare)(e->pool, seq, index, move);
         return rc;
       }
     }

@@ -614,7 +614,7 @@ int32_t b200kv_kv_cache_layer_view(const b200kv_arena* arena, const b200kv_kv_ca
  *   fork          `dst` begins as the first n_tokens of `src` (-1: all) and shares its whole blocks; the half-filled one
  *                 is copied in every layer. Forked sequences are best kept neighbours in `seqs`.
  *   trim          takes back the last n_tokens of a sequence (rejected drafts); a block that others hold and that is
- *                 half filled afterwards is copied first.
+ *                 half filled afterwards is copied, into a free block or, with none left, into one that the call empties.
  *   compact       moves up to max_moves blocks towards the pool's start (-1: all that stand behind a free one);
  *                 returns how many, or a negated error code. fork, trim and compact happen between steps, on the stream of
  *                 the steps before and after; a call that fails changes nothing.
