@@ -11,6 +11,7 @@
 #include <cstring>
 #include <iomanip>
 #include <locale>
+#include <mutex>
 #include <new>
 #include <sstream>
 #include <string>
@@ -37,7 +38,8 @@ struct b200kv_block_pool {
   int32_t* used_blocks;  // table entries in use per sequence
   uint8_t* live;
   int32_t* refs;         // [num_blocks] table entries that name the block: more than one once a sequence has been forked
-  int32_t* scratch;      // [num_blocks] for Validate and for compacting
+  int32_t* scratch;      // [num_blocks] for Validate, the statistics and compacting, under scratch_mutex: who only looks may be another thread
+  mutable std::mutex scratch_mutex;
 };
 
 extern "C" b200kv_block_pool* b200kv_block_pool_create(int32_t num_blocks, int32_t block_size, int32_t max_seqs,
@@ -135,7 +137,7 @@ int32_t RowsIn(const b200kv_block_pool* pool, int32_t seq, int32_t index) {  // 
   return static_cast<int32_t>(left < pool->block_size ? left : pool->block_size);
 }
 
-// scratch[block]: the rows that mean something, those of the sequence with the most tokens there.
+// scratch[block]: the rows that mean something, those of the sequence with the most tokens there. The caller holds scratch_mutex.
 void MarkRows(const b200kv_block_pool* pool) {
   std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
   for (int32_t s = 0; s < pool->max_seqs; ++s) {
@@ -312,6 +314,7 @@ extern "C" int32_t b200kv_block_pool_unshare(b200kv_block_pool* pool, int32_t se
 namespace b200kv {
 // Tokens that the blocks hold, those of several sequences once.
 int64_t StoredTokens(const b200kv_block_pool* pool) {
+  std::lock_guard<std::mutex> lock(pool->scratch_mutex);
   MarkRows(pool);
   int64_t tokens = 0;
   for (int32_t id = 0; id < pool->num_blocks; ++id) tokens += pool->scratch[id];
@@ -362,6 +365,7 @@ extern "C" int32_t b200kv_block_pool_plan_compact(b200kv_block_pool* pool, int32
     SetLastError("plan_compact: %d moves into %p", max_moves, static_cast<void*>(moves_out));
     return moves_out == nullptr ? -B200KV_ERR_NULLPTR : -B200KV_ERR_INVALID;
   }
+  std::lock_guard<std::mutex> lock(pool->scratch_mutex);
   MarkRows(pool);
   int32_t n = 0, to = 0;
   for (int32_t from = pool->num_blocks - 1; n < max_moves; --from) {
@@ -383,6 +387,7 @@ extern "C" int32_t b200kv_block_pool_apply_moves(b200kv_block_pool* pool, const 
     SetLastError("apply_moves: pool and moves must be non-null");
     return B200KV_ERR_NULLPTR;
   }
+  std::lock_guard<std::mutex> lock(pool->scratch_mutex);
   // Plan: sources in use, destinations free, none twice. scratch[id]: 0 untouched, destination + 1 of a source, -1 a destination.
   std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
   for (int32_t i = 0; i < n_moves; ++i) {
@@ -488,6 +493,7 @@ extern "C" int32_t b200kv_block_pool_validate(const b200kv_block_pool* pool) {
     SetLastError("validate: pool is null");
     return B200KV_ERR_NULLPTR;
   }
+  std::lock_guard<std::mutex> lock(pool->scratch_mutex);
   std::memset(pool->scratch, 0, static_cast<size_t>(pool->num_blocks) * sizeof(int32_t));
   int64_t owned = 0;
   int32_t at = pool->head;

@@ -661,7 +661,7 @@ int32_t b200kv_engine_compact(b200kv_engine* engine, int32_t max_moves, void* st
  * lengths and the free list are as before begin_step. */
 int32_t b200kv_engine_abort_step(b200kv_engine* engine);
 /* The "paged_attention" object of the reference's diagnostics for the engine's current state. A token that several sequences share
- * counts once. */
+ * counts once. May be asked from another thread; beside a call that changes the tables the count may be of neither state. */
 int64_t b200kv_engine_stats_json(const b200kv_engine* engine, char* buffer, int64_t capacity);
 
 /* ------------------------------------------------------------------------------------------------
