@@ -83,11 +83,21 @@ struct b200kv_engine {
 namespace {
 
 // From how many common tokens (counted once a pair of neighbours) for each sequence of the step, and from what part of all tokens
-// on, attention goes through the entry point for shared rows. Both sides measured (us a layer, b200kv_mla_decode -> _shared; all
-// sequences share the given length and have 100 tokens of their own): 2 x 512 12.2 -> 12.4, 2 x 1,024 14.0 -> 12.8, 2 x 8,192
-// 23.0 -> 19.7, 4 x 512 12.6 -> 12.9, 4 x 1,024 14.2 -> 14.6, 4 x 4,096 19.6 -> 17.9, 8 x 512 13.4 -> 14.4, 8 x 1,024 17.5 -> 16.9, 8 x 8,192
-// 28.6 -> 24.9, 16 x 512 15.9 -> 17.3, 16 x 1,024 19.4 -> 18.3, 16 x 8,192 39.6 -> 30.5, 32 x 512 17.7 -> 19.9, 32 x 1,024 22.4 -> 21.7,
-// 32 x 2,048 28.3 -> 25.6, 32 x 8,192 61.8 -> 45.7, 32 x 32,768 199 -> 122.
+// on, attention goes through the entry point for shared rows. Both sides measured, us a layer, b200kv_mla_decode -> _shared, over the
+// rows of so many layers that they do not stay in L2; all sequences share the given length and have 100 tokens of their own:
+//           256            512            1,024          2,048          4,096          8,192          32,768
+//     2      9.3 ->  11.8   11.7 ->  11.9   13.3 ->  12.8   17.0 ->  15.7   20.7 ->  17.3   22.3 ->  20.1   29.7 ->  30.3
+//     3      9.3 ->  11.8   11.7 ->  12.1   13.4 ->  14.1   15.2 ->  16.0   16.6 ->  17.6   19.2 ->  21.0   33.6 ->  31.0
+//     4      9.6 ->  12.1   12.0 ->  12.4   13.8 ->  14.5   17.6 ->  15.9   19.0 ->  17.9   21.8 ->  21.2   39.1 ->  32.2
+//     8     11.3 ->  14.2   13.0 ->  15.3   16.9 ->  16.7   17.9 ->  17.5   21.3 ->  19.6   27.8 ->  23.8   61.4 ->  43.5
+//    16     12.7 ->  15.6   15.7 ->  16.8   19.0 ->  18.0   21.0 ->  19.8   27.2 ->  22.9   38.6 ->  29.7   112  ->  70.5
+//    32     14.0 ->  19.3   17.2 ->  19.6   21.9 ->  21.4   27.9 ->  25.3   39.2 ->  32.2   61.1 ->  44.8   219  ->  128
+//    64     16.8 ->  21.8   20.1 ->  24.9   31.7 ->  27.5   43.3 ->  34.8   66.0 ->  47.3   112  ->  71.0   442  ->  241
+//   128     18.0 ->  28.1   41.1 ->  30.3   52.8 ->  37.3   75.6 ->  49.9   120  ->  76.7   230  ->  133
+// Two neighbours are common once, so the line lies between the columns of 512 and 1,024. On its shared side three sequences of up
+// to 8,192 tokens (one of them is alone) lose 4 to 9 %, 4 x 1,024 5 %, 2 x 32,768 2 %; below it 128 x 512 would gain. With out_fp8,
+// which b200kv_mla_decode writes in its merge and the other in a launch of its own, the line would lie higher: 3 x 1,024 .. 8,192 lose 7
+// to 13 %, 4, 8 and 16 sequences up to 4,096 tokens 6 % at most (8 x 2,048 18.6 -> 19.5, 16 x 4,096 28.1 -> 25.6, 32 x 1,024 23.7 -> 23.9).
 constexpr int64_t kLeastCommon = 512;
 constexpr int64_t kCommonPart = 4;
 

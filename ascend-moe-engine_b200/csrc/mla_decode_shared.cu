@@ -33,7 +33,7 @@
 // arriving at 54 bytes a cycle nor shared-memory stores slow them down). A step takes 3,100 to 3,500: S needs T, whose one buffer is
 // filled anew every step, and the softmax of a step (2,400 cycles with the exchange of maxima) stands between its S and its O. Another
 // item costs 2.5 steps more, a call 4.5 us until S comes for the first time, 2.3 us for partials at the rate at which an SM can
-// write, and 7 us for the merge. 128 sequences behind 8,192 common tokens: 134 us (1,120 TFLOP/s), 157 us when they follow one another
+// write, and 7 us for the merge. 128 sequences behind 8,192 common tokens: 134 us (1,120 TFLOP/s), 157 to 160 us when they follow one another
 // for long: the GPU is at its power limit then, with the clock at 1.65 GHz.
 #include <cuda.h>
 
@@ -363,7 +363,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   __syncwarp();
   ptx::ClusterArrive();  // (the barriers are ready: waited for before the peer's are touched)
   if (p.stable_tables == 0) GridDependencyWait();
-  // (let go only after this kernel's own wait: the merge kernel reads the lengths too)
 
   // ---- this run of the list: totals, then the first step at or after the run's first cost position and the next run's ------
   // Each thread has a stretch of the queries: sums over it, one scan over the threads, and those threads that have items of this
@@ -468,6 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   }
+  // (the merge kernel's CTAs may come from here on; they read only what this kernel leaves, and wait for its end)
   GridDependencyTrigger();
   ptx::TcFenceBeforeSync();
   any_empty = __syncthreads_or(any_empty) != 0;

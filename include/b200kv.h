@@ -480,16 +480,16 @@ int32_t b200kv_block_pool_ungrow(b200kv_block_pool* pool, int32_t seq, int32_t n
  *                 many (or a negated error code) and changes nothing. apply_moves changes the tables accordingly, once the copies
  *                 are enqueued; the free list is in the order of the ids afterwards.
  */
-/* What b200kv_shared_args wants to know of a step of one token a sequence: table rows [n_seqs][max_blocks] and lengths in step order
- * (host arrays) -> leader and shared_len [n_seqs], neighbours two by two as the kernel takes them. Returns the common tokens, each
- * pair's counted once, or a negated error code. */
-int64_t b200kv_find_shared(const int32_t* table, int64_t max_blocks, const int32_t* kv_len, int32_t n_seqs, int32_t block_size,
-                           int32_t* leader_out, int32_t* shared_len_out);
 int32_t b200kv_block_pool_fork(b200kv_block_pool* pool, int32_t src, int32_t dst, int32_t n_tokens, int32_t* move_out);
 int32_t b200kv_block_pool_unshare(b200kv_block_pool* pool, int32_t seq, int32_t index, int32_t* move_out);
 int32_t b200kv_block_pool_plan_compact(b200kv_block_pool* pool, int32_t max_moves, int32_t* moves_out);
 int32_t b200kv_block_pool_apply_moves(b200kv_block_pool* pool, const int32_t* moves, int32_t n_moves);
 int32_t b200kv_block_pool_ref_count(const b200kv_block_pool* pool, int32_t block); /* table entries that name it, -1: no such block */
+/* What b200kv_shared_args wants to know of a step of one token a sequence: table rows [n_seqs][max_blocks] and lengths in step order
+ * (host arrays) -> leader and shared_len [n_seqs], neighbours two by two as the kernel takes them. Returns the common tokens, each
+ * pair's counted once, or a negated error code. */
+int64_t b200kv_find_shared(const int32_t* table, int64_t max_blocks, const int32_t* kv_len, int32_t n_seqs, int32_t block_size,
+                           int32_t* leader_out, int32_t* shared_len_out);
 int32_t b200kv_block_pool_free_count(const b200kv_block_pool* pool);
 int32_t b200kv_block_pool_seq_len(const b200kv_block_pool* pool, int32_t seq);
 /* Host views: table [max_seqs][max_blocks_per_seq] (unused entries 0), lens [max_seqs]. */
