@@ -5,7 +5,7 @@
 // steps).
 //
 //   Build      reserve the KV spans and the step's staging in the static arena, note the attention workspace,
-//              ONE commit, the workspace, seal; create the block pool; two pinned staging blocks for the uploads.
+//              ONE commit, the workspace, seal; create the block pool; the uploads' pinned staging blocks.
 //   step       begin: grow every sequence of the step in the block pool (plan, then commit: a refused growth
 //              changes nothing), write the step's table rows, lengths and slots into a pinned block and upload
 //              them with ONE copy (the reference's mailbox, :515-519). Then per layer, in the reference's stage
@@ -65,6 +65,9 @@ struct b200kv_engine {
   static constexpr int kStagings = 2;
   Staging stagings[kStagings];
   int at_staging = 0;
+  // What an upload that is part of a graph reads when the graph runs: the step begun last, from the first such upload on.
+  unsigned char* captured = nullptr;
+  bool has_captured = false;
   unsigned char* staging = nullptr;  // of the step in hand
   size_t staging_bytes = 0;
   size_t table_off = 0, slots_off = 0, lens_off = 0;
@@ -154,23 +157,26 @@ int32_t TakeStaging(b200kv_engine* e) {
   return B200KV_OK;
 }
 
-// The block in hand goes to the device, from byte `from` on. An upload that becomes part of a graph is read when the graph runs and
-// leaves no event.
+// The block in hand goes to the device, from byte `from` on.
 int32_t Upload(b200kv_engine* e, size_t from, cudaStream_t stream) {
   unsigned char* to = reinterpret_cast<unsigned char*>(e->d_queries) + from;
+  const size_t bytes = e->staging_bytes - from;
   if (int32_t rc = b200kv::FaultCheck("b200kv_engine_step_upload")) return rc;
   if (e->cfg.backend != B200KV_ARENA_DEVICE) {
-    std::memcpy(to, e->staging + from, e->staging_bytes - from);
-  } else {
-    b200kv_engine::Staging& block = e->stagings[e->at_staging];
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (int32_t rc = CheckCuda(cudaStreamIsCapturing(stream, &capture), "engine step upload")) return rc;
-    if (int32_t rc = CheckCuda(cudaMemcpyAsync(to, e->staging + from, e->staging_bytes - from, cudaMemcpyHostToDevice, stream), "engine step upload")) return rc;
-    if (capture == cudaStreamCaptureStatusNone) {
-      if (int32_t rc = CheckCuda(cudaEventRecord(block.uploaded, stream), "engine step upload")) return rc;
-      block.pending = true;
-    }
+    std::memcpy(to, e->staging + from, bytes);
+    return B200KV_OK;
   }
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (int32_t rc = CheckCuda(cudaStreamIsCapturing(stream, &capture), "engine step upload")) return rc;
+  e->has_captured |= capture != cudaStreamCaptureStatusNone;
+  if (e->has_captured) std::memcpy(e->captured, e->staging, e->staging_bytes);
+  if (capture != cudaStreamCaptureStatusNone) {
+    return CheckCuda(cudaMemcpyAsync(to, e->captured + from, bytes, cudaMemcpyHostToDevice, stream), "engine step upload");
+  }
+  b200kv_engine::Staging& block = e->stagings[e->at_staging];
+  if (int32_t rc = CheckCuda(cudaMemcpyAsync(to, block.at + from, bytes, cudaMemcpyHostToDevice, stream), "engine step upload")) return rc;
+  if (int32_t rc = CheckCuda(cudaEventRecord(block.uploaded, stream), "engine step upload")) return rc;
+  block.pending = true;
   e->at_staging = (e->at_staging + 1) % b200kv_engine::kStagings;
   return B200KV_OK;
 }
@@ -265,18 +271,26 @@ extern "C" b200kv_engine* b200kv_engine_create(const b200kv_engine_config* confi
   e->slots_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.slot_mapping_handle) - first);
   e->lens_off = static_cast<size_t>(b200kv_arena_offset(e->arena, e->cache.seq_lens_handle) - first);
   e->staging_bytes = e->lens_off + static_cast<size_t>(c.max_seqs) * 4;
-  for (b200kv_engine::Staging& block : e->stagings) {
+  auto host_block = [&](unsigned char** at) -> bool {
     if (c.backend == B200KV_ARENA_DEVICE) {
       void* pinned = nullptr;
-      if (CheckCuda(cudaMallocHost(&pinned, e->staging_bytes), "engine staging (pinned)") != B200KV_OK) return fail();
-      block.at = static_cast<unsigned char*>(pinned);
-      if (CheckCuda(cudaEventCreateWithFlags(&block.uploaded, cudaEventDisableTiming), "engine staging (event)") != B200KV_OK) return fail();
+      if (CheckCuda(cudaMallocHost(&pinned, e->staging_bytes), "engine staging (pinned)") != B200KV_OK) return false;
+      *at = static_cast<unsigned char*>(pinned);
     } else {
-      block.at = new (std::nothrow) unsigned char[e->staging_bytes];
-      if (block.at == nullptr) return fail();
+      *at = new (std::nothrow) unsigned char[e->staging_bytes];
+      if (*at == nullptr) return false;
     }
-    std::memset(block.at, 0, e->staging_bytes);
+    std::memset(*at, 0, e->staging_bytes);
+    return true;
+  };
+  for (b200kv_engine::Staging& block : e->stagings) {
+    if (!host_block(&block.at)) return fail();
+    if (c.backend == B200KV_ARENA_DEVICE &&
+        CheckCuda(cudaEventCreateWithFlags(&block.uploaded, cudaEventDisableTiming), "engine staging (event)") != B200KV_OK) {
+      return fail();
+    }
   }
+  if (!host_block(&e->captured)) return fail();
   e->pool = b200kv_block_pool_create(c.num_blocks, c.block_size, c.max_seqs, c.max_blocks_per_seq, nullptr);
   if (e->pool == nullptr) return fail();
   e->step_seq_ids.resize(static_cast<size_t>(c.max_seqs));
@@ -289,11 +303,15 @@ extern "C" b200kv_engine* b200kv_engine_create(const b200kv_engine_config* confi
 extern "C" void b200kv_engine_destroy(b200kv_engine* e) {
   if (e == nullptr) return;
   if (e->pool != nullptr) b200kv_block_pool_destroy(e->pool);
+  auto free_block = [&](unsigned char* at) {
+    if (at == nullptr) return;
+    if (e->cfg.backend == B200KV_ARENA_DEVICE) cudaFreeHost(at); else delete[] at;
+  };
   for (b200kv_engine::Staging& block : e->stagings) {
     if (block.uploaded != nullptr) cudaEventDestroy(block.uploaded);
-    if (block.at == nullptr) continue;
-    if (e->cfg.backend == B200KV_ARENA_DEVICE) cudaFreeHost(block.at); else delete[] block.at;
+    free_block(block.at);
   }
+  free_block(e->captured);
   if (e->arena != nullptr) b200kv_arena_destroy(e->arena);
   delete e;
 }

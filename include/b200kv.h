@@ -596,15 +596,16 @@ int32_t b200kv_kv_cache_layer_view(const b200kv_arena* arena, const b200kv_kv_ca
  * of many tokens where the reference keeps one sequence and one token per step
  * (src/memory/static_arena_manager.cpp:37-39; src/pipeline/pipeline.cpp:40, 515-519; apps/moe_runner.cpp:434-439).
  *   create        Build: the KV spans reserved in a static arena, the attention workspace noted, one Commit, the
- *                 workspace, Seal; the block pool; two pinned blocks for the per-step upload. Nothing allocates
- *                 afterwards.
+ *                 workspace, Seal; the block pool; the pinned blocks for the per-step upload. Nothing
+ *                 allocates afterwards.
  *   admit/release a sequence enters with no tokens / leaves and its blocks return to the free list.
  *   begin_step    seqs[i] grows by new_tokens[i] tokens (null: one each, a decode step; more: a prefill chunk).
  *                 Plan, then commit: a step that does not fit (tokens per step, blocks per sequence, free blocks)
  *                 is refused and changes nothing. The step's table rows (row i = seqs[i]), lengths and slots go
  *                 to the device with ONE copy (the reference's slot mailbox, :515-519). Steps may be enqueued one
  *                 behind the other: a step's call waits until the upload of the step before the last has been made. (An
- *                 upload that is captured into a graph is read when the graph runs: before the second step after it begins.)
+ *                 upload that is captured into a graph uploads, whenever the graph runs, the step begun last: wait for the
+ *                 graph before the next step begins.)
  *   layer_append  stages 6-8 of the reference's layer (kv_a_norm, rope, kv_cache_write) for the step's new tokens,
  *                 rows in step order (all tokens of seqs[0], then seqs[1], ...): b200kv_append_fused.
  *   layer_attend  stage 9 (attention of the step's new tokens, each over its sequence up to itself) and, when out_fp8

@@ -144,7 +144,32 @@ def test_a_step_captured_as_a_whole_between_eager_ones():
     with torch.cuda.graph(graph):   # (takes the block of the first step, whose upload left an event)
         a.step(*steps[2], made[2])
     graph.replay()
+    torch.cuda.synchronize()        # the graph has read the step
     a.step(*steps[3], made[3])
-    torch.cuda.synchronize()        # the graph has read its block
     a.step(*steps[4], made[4])
     a.check()
+
+
+def test_a_captured_step_uploads_the_step_begun_last():
+    """The graph of a decode step, run again for later steps, whose growth an eager call has planned."""
+    a = Ahead()
+    a.admit(0, 1)
+    steps = [([0, 1], [63, 130]), ([0, 1], [1, 1])]
+    made = a.inputs(steps)
+    a.step(*steps[0], made[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(*steps[1], made[1])
+    for i in range(4):
+        if i > 0:
+            a.e.begin_step([0, 1])
+            for l, (kv_a, q, out) in enumerate(made[1]):
+                for k, s in enumerate((0, 1)):
+                    a.rows[s][l].append(kv_a[k])
+            a.e.end_step()
+        graph.replay()
+        torch.cuda.synchronize()
+        if i > 0:
+            a.done = [(l, s, len(a.rows[s][l]) - 1, g, q, out) for l, s, _, g, q, out in a.done if g == 1]
+        a.check()
